@@ -105,6 +105,28 @@ SIGNATURES = {
         _I,
         [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I64, _P],
     ),
+    "d3d_kv_append_fp8": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "d3d_qk_rope_append_fp8": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P],
+    ),
+    "d3d_qk_rope_append_fp8_parts": (
+        _I,
+        [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P],
+    ),
+    "d3d_attn_fp8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    "d3d_verify_attn_paged_fp8": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P],
+    ),
+    "d3d_draft_block_attn_fp8": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P],
+    ),
+    "d3d_packed_block_attn_fp8": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P],
+    ),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -578,6 +578,83 @@ int d3d_qk_rope_append_parts(const float* parts, int splits, const int64_t* posi
                              void* v_cache, const int64_t* slot_mapping, int T, int Hq, int Hkv, int D,
                              float eps, int draft_rope, int64_t num_slots, void* stream);
 
+/*
+ * The 8-bit paged KV cache.  Codes: k_cache, v_cache [num_pages, Hkv,
+ * page_size, 128] e4m3 (head-major pages: a (page, head) is contiguous),
+ * 16-byte aligned.  Scales: k_scale, v_scale [num_pages, Hkv, page_size /
+ * block], one byte for each block of `block` tokens of a page and KV head,
+ * scale = 2^(byte - 127) (e8m0).  An entry stands for code * scale.  block is
+ * a power of two in 16 .. 256 that divides page_size (D3D_E_UNSUPPORTED
+ * otherwise); flat slot s is slot s % page_size of page s / page_size.  A cache
+ * of zero bytes is a valid empty one.
+ *
+ * Appends follow one rule per touched block and KV head, keys and values
+ * apart.  need = the least e in [-117, 119] with amax(finite new entries) <=
+ * 448 * 2^e.  If the call writes the block's first slot, e = need and the
+ * slots that the call does not write become 0: the block starts anew, so pages
+ * can be used again without clearing.  Otherwise e = max(old e, need), and the
+ * kept codes become e4m3(code * 2^(old e - e)), exact unless they leave the
+ * normal range.  New codes are e4m3(x * 2^-e), to nearest even; entries past
+ * 448 * 2^119 saturate, NaN and infinities are stored as NaN.  Tokens may
+ * come in any order; of tokens with the same slot the last one counts, and
+ * slots outside [0, num_pages * page_size) are skipped.
+ *
+ * d3d_kv_append_fp8: k, v bf16, rows of Hkv * 128 entries k_stride / v_stride
+ * entries apart (multiples of 4; rows 8-byte aligned).
+ */
+int d3d_kv_append_fp8(const void* k, const void* v, int64_t k_stride, int64_t v_stride, void* k_cache, void* v_cache,
+                      void* k_scale, void* v_scale, const int64_t* slot_mapping, int n_tokens, int Hkv, int D,
+                      int page_size, int block, int num_pages, void* stream);
+
+/*
+ * d3d_qk_rope_append over the 8-bit cache: q and k heads get RMSNorm over D
+ * and rotate-half RoPE, q goes to q_out [T, Hq, 128] bf16, k and v into the
+ * cache at slot_mapping[t].  Norm, rotation and scaling run in fp32 with one
+ * rounding at the end (q to bf16, k to its code); angles positions[t] *
+ * inv_freq[i] are reduced in 64 bits, so far positions lose nothing.  qkv, the
+ * norm weights and q_out 8-byte aligned, inv_freq and parts 16-byte.
+ * The _parts form takes qkv as the partials of d3d_gemm_rows64 (summed in
+ * split order and rounded to bf16), as d3d_qk_rope_append_parts does.
+ */
+int d3d_qk_rope_append_fp8(const void* qkv, const int64_t* positions, const void* q_norm_w, const void* k_norm_w,
+                           const float* inv_freq, void* q_out, void* k_cache, void* v_cache, void* k_scale,
+                           void* v_scale, const int64_t* slot_mapping, int T, int Hq, int Hkv, int D, float eps,
+                           int page_size, int block, int num_pages, void* stream);
+int d3d_qk_rope_append_fp8_parts(const float* parts, int splits, const int64_t* positions, const void* q_norm_w,
+                                 const void* k_norm_w, const float* inv_freq, void* q_out, void* k_cache,
+                                 void* v_cache, void* k_scale, void* v_scale, const int64_t* slot_mapping, int T,
+                                 int Hq, int Hkv, int D, float eps, int page_size, int block, int num_pages,
+                                 void* stream);
+
+/* Bytes of workspace the attention calls over the 8-bit cache need; max_context
+ * bounds every context_lens[b] and is passed to the call as well. */
+size_t d3d_attn_fp8_workspace_bytes(int B, int Q, int Hq, int Hkv, int D, int page_size, int max_context);
+
+/*
+ * Block attention over the 8-bit cache: d3d_verify_attn_paged,
+ * d3d_draft_block_attn and d3d_packed_block_attn with the cache's codes and
+ * scales.  q and out bf16, 16-byte aligned.  A row that sees no key is 0.  A key
+ * or value that holds a NaN reaches only the rows that see it; what lies
+ * behind a context, in pages past it or in keys that a row does not see, has no
+ * influence.  Page ids outside [0, num_pages) read as zero keys and values;
+ * keys at or past max_context are not read.
+ */
+int d3d_verify_attn_paged_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+                              const void* v_scale, const int32_t* block_table, const int32_t* context_lens, void* out,
+                              int B, int Q, int Hq, int Hkv, int D, int page_size, int block, int max_pages,
+                              int num_pages, float scale, int max_context, void* workspace, size_t workspace_bytes,
+                              void* stream);
+int d3d_draft_block_attn_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+                             const void* v_scale, const int32_t* block_table, const int32_t* context_lens, void* out,
+                             int B, int Q, int Hq, int Hkv, int D, int page_size, int block, int max_pages,
+                             int num_pages, float scale, int max_context, void* workspace, size_t workspace_bytes,
+                             void* stream);
+int d3d_packed_block_attn_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+                              const void* v_scale, const int32_t* block_table, const int32_t* context_lens,
+                              const int32_t* q_visibility, void* out, int B, int Q, int Hq, int Hkv, int D,
+                              int page_size, int block, int max_pages, int num_pages, float scale, int max_context,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

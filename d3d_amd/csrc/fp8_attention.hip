@@ -38,8 +38,16 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
+#ifndef SL1
+#define SL1 512
+#define SL2 512
+#define SL4 512
+#define MT1 2
+#define MT2 2
+#define MT4 2
+#endif
 constexpr int kStep = 32;       // tokens a wave takes at a time
 constexpr int kTile = 128;      // tokens four waves take at a time: the unit of ranges
 constexpr int kMaxTiles = 64;   // tiles of a range whose pages and scales are staged at once
@@ -59,10 +67,12 @@ struct AttnParams {
     _Float16* part_o;  // [item][nqt][Hkv][M][D], O / l of a range, times 2^-e
     f32x4* part_ml;    // [item][nqt][Hkv][M]: m, l, 2^e of dims 0..63, of 64..127
     int B, Q, Hq, Hkv, G, QT, nqt, M;
+    int qt_inv;      // 2^16 / QT rounded up: row / QT of rows below 64
+    int page_shift;  // log2 of the page size, or -1
     int page_size, block_shift, max_pages, num_pages;
     int max_context;
     int items;   // ranges of all requests at most
-    int slots;   // workgroups that run at once
+    int room;    // ranges that run at once
     int min_tiles;  // tiles per range at least
     int dense;   // ranges per request when items are not packed (B > 64), else 0
     int dense_tiles;
@@ -76,81 +86,89 @@ __device__ __forceinline__ int ctx_of(const AttnParams& P, int b) {
 }
 
 __device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v += xor_desc<32>(v);
+    v += xor_desc<16>(v);
+    v += xor_desc<8>(v);
+    v += xor_desc<4>(v);
+    v += xor_desc<2>(v);
+    return v + xor_desc<1>(v);
 }
 
-// How the context is cut, the same in every workgroup of both launches.  Up to
-// 64 requests: ranges of `tiles` whole tiles, the least number of tiles that
-// keeps the ranges of all requests within P.slots workgroups; item numbers
-// run through the requests' own range counts.  A whole wave calls it.
+template <int O>
+__device__ __forceinline__ int scan_step(int v, int lane) {
+    const int t = (int)up_partner<O>((uint32_t)v);
+    return lane >= O ? v + t : v;
+}
+
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// How the contexts are cut, the same in every workgroup of both launches.  Up
+// to 64 requests: with the least number of tiles per range that keeps the
+// ranges of all requests within P.slots workgroups; item numbers run through
+// the requests' own range counts.  A whole wave calls it.
 struct Range {
-    int b, s, n, tiles, first;  // request (-1: none), range, ranges of the request, tiles per range, its first item
+    int b, s, n, first;  // request (-1: none), range, ranges of the request, its first item
 };
 
-__device__ __forceinline__ void cut_of(const AttnParams& P, int lane, int& tiles, int& incl, int& n) {
-    const int t = lane < P.B ? (max(ctx_of(P, lane), 1) + kTile - 1) / kTile : 0;
-    const int per = P.Hkv * P.nqt, room = max(P.slots / per, 1);
+__device__ __forceinline__ int tiles_of(const AttnParams& P, int b) {
+    return (max(ctx_of(P, b), 1) + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ void cut_of(const AttnParams& P, int lane, int& incl, int& n) {
+    const int t = lane < P.B ? tiles_of(P, lane) : 0;
     const int total = wave_sum_int(t);
-    tiles = max(P.min_tiles, (total + room - 1) / room);
+    int tiles = max(P.min_tiles, (total + P.room - 1) / P.room);
     for (;;) {
         n = lane < P.B ? (t + tiles - 1) / tiles : 0;
         const int sum = wave_sum_int(n);
-        if (sum <= max(room, P.B)) break;  // one range each at the least
-        tiles += max(1, tiles * (sum - room) / (2 * sum));
+        if (sum <= max(P.room, P.B)) break;  // one range each at the least
+        tiles += max(1, tiles * (sum - P.room) / (2 * sum));
     }
-    incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += u;
-    }
+    incl = scan_step<1>(n, lane);
+    incl = scan_step<2>(incl, lane);
+    incl = scan_step<4>(incl, lane);
+    incl = scan_step<8>(incl, lane);
+    incl = scan_step<16>(incl, lane);
+    incl = scan_step<32>(incl, lane);
+}
+
+// One request: the same, without the wave.
+__device__ __forceinline__ int cut_of_one(const AttnParams& P) {
+    const int t = tiles_of(P, 0), tiles = max(P.min_tiles, (t + P.room - 1) / P.room);
+    return (t + tiles - 1) / tiles;
+}
+
+__device__ __forceinline__ int cut_dense(const AttnParams& P, int b) {
+    return (tiles_of(P, b) + P.dense_tiles - 1) / P.dense_tiles;
 }
 
 __device__ __forceinline__ Range range_of_item(const AttnParams& P, int item) {
-    Range r;
     if (P.dense) {
-        r.b = P.B - 1 - item / P.dense;  // later requests first: a prompt's longer slices
-        r.s = item % P.dense;
-        r.tiles = P.dense_tiles;
-        r.n = max(1, (ctx_of(P, r.b) + kTile * r.tiles - 1) / (kTile * r.tiles));
-        r.first = item - r.s;
-        if (r.s >= r.n) r.b = -1;
-        return r;
+        const int b = P.B - 1 - item / P.dense, s = item % P.dense;  // later requests first: a prompt's longer slices
+        const int n = cut_dense(P, b);
+        return {s < n ? b : -1, s, n, item - s};
+    }
+    if (P.B == 1) {
+        const int n = cut_of_one(P);
+        return {item < n ? 0 : -1, item, n, 0};
     }
     const int lane = threadIdx.x & 63;
     int incl, n;
-    cut_of(P, lane, r.tiles, incl, n);
+    cut_of(P, lane, incl, n);
     const uint64_t past = __ballot(lane < P.B && incl > item);
-    if (!past) {
-        r.b = -1;
-        r.s = r.n = r.first = 0;
-        return r;
-    }
-    r.b = __builtin_ctzll(past);
-    r.n = __shfl(n, r.b, 64);
-    r.first = __shfl(incl, r.b, 64) - r.n;
-    r.s = item - r.first;
-    return r;
+    if (!past) return {-1, 0, 0, 0};
+    const int b = __builtin_ctzll(past), nb = lane_value(n, b), first = lane_value(incl, b) - nb;
+    return {b, item - first, nb, first};
 }
 
 __device__ __forceinline__ Range range_of_request(const AttnParams& P, int b) {
-    Range r;
-    r.b = b;
-    r.s = 0;
-    if (P.dense) {
-        r.tiles = P.dense_tiles;
-        r.n = max(1, (ctx_of(P, b) + kTile * r.tiles - 1) / (kTile * r.tiles));
-        r.first = (P.B - 1 - b) * P.dense;
-        return r;
-    }
+    if (P.dense) return {b, 0, cut_dense(P, b), (P.B - 1 - b) * P.dense};
+    if (P.B == 1) return {0, 0, cut_of_one(P), 0};
     const int lane = threadIdx.x & 63;
     int incl, n;
-    cut_of(P, lane, r.tiles, incl, n);
-    r.n = __shfl(n, b, 64);
-    r.first = __shfl(incl, b, 64) - r.n;
-    return r;
+    cut_of(P, lane, incl, n);
+    const int nb = lane_value(n, b);
+    return {b, 0, nb, lane_value(incl, b) - nb};
 }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
@@ -190,16 +208,20 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 }
 
 template <int MODE, int RT, int NW>
-__global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnParams P) {
+__global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     constexpr int NT = NW * 64, R = 16 * RT;
     constexpr int kGroups = kMaxTiles * kTile / 16;
     // Output exchange: half the dimensions at a time, a row's floats padded.
     constexpr int kHalf = D / 2, kORow = kHalf + 4;
-    constexpr int kVBytes = NW * kStep * kVRow, kOBytes = NW * R * kORow * 4;
-    __shared__ __attribute__((aligned(16))) char lds[kVBytes > kOBytes ? kVBytes : kOBytes];
-    __shared__ int row_of[kGroups];       // first cache row of a 16-token group, -1: no page
-    __shared__ u32x2 scale_of[kGroups];   // its key and value scales
+    // Four row tiles' query operands stay in LDS: with them in registers too, one
+    // wave fits a SIMD instead of two.
+    constexpr bool QLDS = RT == 4;
+    constexpr int kVBytes = NW * kStep * kVRow, kQBytes = QLDS ? RT * 4 * 64 * 16 : 0, kOBytes = NW * R * kORow * 4;
+    __shared__ __attribute__((aligned(16))) char lds[kVBytes + kQBytes > kOBytes ? kVBytes + kQBytes : kOBytes];
+    __shared__ int row_of[kGroups];      // first cache row of a 16-token group, -1: no page
+    __shared__ u32x2 scale_of[kGroups];  // its key and value scales
     __shared__ float stat[2][NW][R];
+    __shared__ int limit[MODE == kPacked ? 3 : 1][R];  // per row: visible keys t < [0], [1] <= t < [2]
 
     const int kvh = blockIdx.x % P.Hkv, qt = blockIdx.y, item = blockIdx.x / P.Hkv;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -207,66 +229,81 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
     const Range rg = range_of_item(P, item);
     const int b = __builtin_amdgcn_readfirstlane(rg.b);
     if (b < 0) return;  // uniform, before any barrier
-    const int ctx = ctx_of(P, b), q0 = qt * P.QT;
-    const int t_begin = __builtin_amdgcn_readfirstlane(rg.s) * __builtin_amdgcn_readfirstlane(rg.tiles) * kTile;
+    const int n_ranges = __builtin_amdgcn_readfirstlane(rg.n);
+    const int len = __builtin_amdgcn_readfirstlane(min(P.context_lens[b], P.max_pages * P.page_size));
+    const int ctx = min(len, P.max_context), pre = len - P.Q, q0 = qt * P.QT;
+    // The request's tiles in n_ranges even parts.
+    const uint64_t tiles = (uint64_t)((max(ctx, 1) + kTile - 1) / kTile), s_r = (uint64_t)__builtin_amdgcn_readfirstlane(rg.s);
+    const int t_begin = (int)(s_r * tiles / n_ranges) * kTile;
+    const int t_last = min((int)((s_r + 1) * tiles / n_ranges) * kTile, ctx);
 
-    // This lane's rows: head gh of the group, query qi; visible keys t < va, vlo <= t < vhi.
-    int qi[RT], head[RT], va[RT], vlo[RT], vhi[RT];
-    bool row_ok[RT];
+    // This lane's rows: head gh of the group, query qi.  The frontier goes by the
+    // context's own length, reads by its bounds.
+    bf16x8 qop[QLDS ? 1 : RT][4];
     int a_min = INT_MAX, a_max = 0, s_lo = INT_MAX, s_hi = 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int row = rt * 16 + c16, gh = row / P.QT;
-        qi[rt] = q0 + row - gh * P.QT;
-        row_ok[rt] = row < P.M && qi[rt] < P.Q;
-        head[rt] = kvh * P.G + (row_ok[rt] ? gh : 0);
-        va[rt] = vlo[rt] = vhi[rt] = 0;
-        if (row_ok[rt]) {
-            // The frontier goes by the context's own length, reads by its bounds.
-            const int pre = min(P.context_lens[b], P.max_pages * P.page_size) - P.Q;
-            va[rt] = ctx;
-            if constexpr (MODE == kCausal) va[rt] = pre + qi[rt] + 1;
+        const int row = rt * 16 + c16, gh = row * P.qt_inv >> 16, qi = q0 + row - gh * P.QT;
+        const bool row_ok = row < P.M && qi < P.Q;
+        // Q^T operands: dims 64 p + 16 g4 + 8 e .. + 7 at ks = 2 p + e, as the keys are loaded.
+        if (!QLDS || rt % NW == w) {
+            const uint16_t* src = P.q + (((size_t)b * P.Q + (row_ok ? qi : 0)) * P.Hq + kvh * P.G + (row_ok ? gh : 0)) * D + 16 * g4;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                u32x4 v = *reinterpret_cast<const u32x4*>(src + 64 * (ks >> 1) + 8 * (ks & 1));
+                if (!row_ok) v = u32x4{0u, 0u, 0u, 0u};
+                if constexpr (QLDS)
+                    *reinterpret_cast<u32x4*>(lds + kVBytes + ((rt * 4 + ks) * 64 + lane) * 16) = v;
+                else
+                    qop[rt][ks] = __builtin_bit_cast(bf16x8, v);
+            }
+        }
+        int va = 0, lo = 0, hi = 0;
+        if (row_ok) {
+            va = ctx;
+            if constexpr (MODE == kCausal) va = min(pre + qi + 1, ctx);
             if constexpr (MODE == kPacked) {
-                va[rt] = pre + P.vis[qi[rt] * 3];
-                vlo[rt] = max(pre + P.vis[qi[rt] * 3 + 1], 0);
-                vhi[rt] = min(pre + P.vis[qi[rt] * 3 + 2], ctx);
+                va = min(pre + P.vis[qi * 3], ctx);
+                lo = max(pre + P.vis[qi * 3 + 1], 0);
+                hi = min(pre + P.vis[qi * 3 + 2], ctx);
+                a_min = min(a_min, va);
+                a_max = max(a_max, va);
+                if (lo < hi) {
+                    s_lo = min(s_lo, lo);
+                    s_hi = max(s_hi, hi);
+                }
             }
-            va[rt] = min(va[rt], ctx);
-            a_min = min(a_min, va[rt]);
-            a_max = max(a_max, va[rt]);
-            if (MODE == kPacked && vlo[rt] < vhi[rt]) {
-                s_lo = min(s_lo, vlo[rt]);
-                s_hi = max(s_hi, vhi[rt]);
+        }
+        // Every wave has the same rows; they are read where a step has keys that
+        // some row does not see, which leaves the registers to the main loop.
+        if (g4 == 0 && w == 0) {
+            limit[0][row] = va;
+            if constexpr (MODE == kPacked) {
+                limit[1][row] = lo;
+                limit[2][row] = hi;
             }
         }
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        a_min = min(a_min, __shfl_xor(a_min, o, 64));
-        a_max = max(a_max, __shfl_xor(a_max, o, 64));
-        if constexpr (MODE == kPacked) {
-            s_lo = min(s_lo, __shfl_xor(s_lo, o, 64));
-            s_hi = max(s_hi, __shfl_xor(s_hi, o, 64));
-        }
+    // Over all rows: keys below a_min are seen by each, none from a_max on by any but [s_lo, s_hi).
+    if constexpr (MODE == kPacked) {
+        const auto all = [](int& v, auto f) {
+            v = f(v, xor_desc<8>(v));
+            v = f(v, xor_desc<4>(v));
+            v = f(v, xor_desc<2>(v));
+            v = __builtin_amdgcn_readfirstlane(f(v, xor_desc<1>(v)));
+        };
+        const auto lo = [](int x, int y) { return min(x, y); };
+        const auto hi = [](int x, int y) { return max(x, y); };
+        all(a_min, lo);
+        all(a_max, hi);
+        all(s_lo, lo);
+        all(s_hi, hi);
+    } else if constexpr (MODE == kCausal) {
+        a_min = min(pre + q0 + 1, ctx);
+        a_max = min(pre + min(q0 + P.QT, P.Q), ctx);
+    } else {
+        a_min = a_max = ctx;
     }
-    a_min = __builtin_amdgcn_readfirstlane(a_min);
-    a_max = __builtin_amdgcn_readfirstlane(a_max);
-    s_lo = __builtin_amdgcn_readfirstlane(s_lo);
-    s_hi = __builtin_amdgcn_readfirstlane(s_hi);
-    const int t_last = min(t_begin + __builtin_amdgcn_readfirstlane(rg.tiles) * kTile, ctx);
-
-    // Q^T operands: dims 64 p + 16 g4 + 8 e .. + 7 at ks = 2 p + e, as the keys are loaded.
-    bf16x8 qop[RT][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (row_ok[rt])
-                v = *reinterpret_cast<const u32x4*>(P.q + (((size_t)b * P.Q + qi[rt]) * P.Hq + head[rt]) * D +
-                                                    64 * (ks >> 1) + 16 * g4 + 8 * (ks & 1));
-            qop[rt][ks] = __builtin_bit_cast(bf16x8, v);
-        }
 
     f32x4 o[RT][8];
     float m[RT], l[RT];
@@ -278,6 +315,7 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
         l[rt] = 0.f;
     }
 
+    bool first = true;  // nothing to rescale yet
     char* vbuf = lds + w * (kStep * kVRow);
     // The value row that this lane stores: token j 8 + lane / 8 goes to row 8 g +
     // 4 sub + r (token 16 sub + 4 g + r), so that a group's eight are neighbours.
@@ -303,42 +341,58 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
         const auto step_at = [&](int j) { return j < n1 ? j : st2 + j - n1; };
         __syncthreads();  // the tables of the piece before are no longer read
         const int groups = 2 * (step_at(steps - 1) + 1);
-        for (int i = threadIdx.x; i < groups; i += NT) {
-            const int t = p0 + 16 * i;
-            int row = -1;
-            u32x2 sc = {0x3f800000u, 0x3f800000u};
-            if (t < p_end) {
-                const int pi = t / P.page_size, in = t - pi * P.page_size;
+        constexpr int kPer = kGroups / NT;
+        int row[kPer];
+        size_t at[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int i = threadIdx.x + k * NT, t = p0 + 16 * i;
+            row[k] = -1;
+            at[k] = 0;
+            if (i < groups && t < p_end) {
+                const int pi = P.page_shift >= 0 ? t >> P.page_shift : t / P.page_size, in = t - pi * P.page_size;
                 const int page = P.block_table[(size_t)b * P.max_pages + pi];
                 if (page >= 0 && page < P.num_pages) {
                     const size_t ph = (size_t)page * P.Hkv + kvh;
-                    const size_t at = ph * (P.page_size >> P.block_shift) + (in >> P.block_shift);
-                    row = (int)(ph * P.page_size + in);
-                    sc[0] = (uint32_t)P.k_scale[at] << 23;
-                    sc[1] = (uint32_t)P.v_scale[at] << 23;
+                    at[k] = ph * (P.page_size >> P.block_shift) + (in >> P.block_shift);
+                    row[k] = (int)(ph * P.page_size + in);
                 }
             }
-            row_of[i] = row;
-            scale_of[i] = sc;
+            if (i < groups) row_of[i] = row[k];
         }
         __syncthreads();
 
         u32x4 kr[2][2], vr[4];
-        const auto fetch = [&](int j) {
-            const int g = 2 * step_at(j);
+        const auto base_of = [&](int g) { return (size_t)max(__builtin_amdgcn_readfirstlane(row_of[g]), 0) * D; };
+        const auto fetch_k = [&](int j) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-                const int row = max(__builtin_amdgcn_readfirstlane(row_of[g + sub]), 0);
-                const uint8_t* kb = P.k_cache + (size_t)row * D;
-                const uint8_t* vb = P.v_cache + (size_t)row * D;
+                const uint8_t* src = P.k_cache + base_of(2 * step_at(j) + sub);
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    kr[sub][p] = *reinterpret_cast<const u32x4*>(kb + k_off + 64 * p);
-                    vr[2 * sub + p] = *reinterpret_cast<const u32x4*>(vb + v_off + 8 * D * p);
-                }
+                for (int p = 0; p < 2; ++p) kr[sub][p] = *reinterpret_cast<const u32x4*>(src + k_off + 64 * p);
             }
         };
-        if (w < steps) fetch(w);
+        const auto fetch_v = [&](int j) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                const uint8_t* src = P.v_cache + base_of(2 * step_at(j) + sub);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) vr[2 * sub + p] = *reinterpret_cast<const u32x4*>(src + v_off + 8 * D * p);
+            }
+        };
+        if (w < steps) {
+            fetch_k(w);
+            fetch_v(w);
+        }
+        // The scales come beside the first keys and values.
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int i = threadIdx.x + k * NT;
+            if (i < groups)
+                scale_of[i] = row[k] < 0 ? u32x2{0x3f800000u, 0x3f800000u}
+                                         : u32x2{(uint32_t)P.k_scale[at[k]] << 23, (uint32_t)P.v_scale[at[k]] << 23};
+        }
+        __syncthreads();
         for (int j = w; j < steps; j += NW) {
             const int t0 = p0 + kStep * step_at(j), g = 2 * step_at(j);
             const bool ok0 = __builtin_amdgcn_readfirstlane(row_of[g]) >= 0;
@@ -380,7 +434,6 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
                 kf[1][2 * p] = widen8(kr[1][p][0], kr[1][p][1], ks1, ks1);
                 kf[1][2 * p + 1] = widen8(kr[1][p][2], kr[1][p][3], ks1, ks1);
             }
-            if (j + NW < steps) fetch(j + NW);
 
             // sc[rt][sub][r]: token t0 + 16 sub + 4 g4 + r, row c16 of row tile rt.
             f32x4 sc[RT][2];
@@ -389,21 +442,42 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-                        sc[rt][sub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[sub][ks], qop[rt][ks], sc[rt][sub], 0, 0, 0);
-            if (edge) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+                for (int rt = 0; rt < RT; ++rt) {
+                    bf16x8 qf;
+                    if constexpr (QLDS)
+                        qf = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(lds + kVBytes + ((rt * 4 + ks) * 64 + lane) * 16));
+                    else
+                        qf = qop[rt][ks];
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub)
+                        sc[rt][sub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[sub][ks], qf, sc[rt][sub], 0, 0, 0);
+                }
+            // The next step's loads: not before the keys' registers are free (earlier
+            // the compiler spills them, and waits for them to do so: 131,072-token
+            // contexts 142 us instead of 104).
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + NW < steps) {
+                fetch_k(j + NW);
+                fetch_v(j + NW);
+            }
+            if (edge) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int row = 16 * rt + c16, va = min(limit[0][row], p_end);
+                    const int lo = MODE == kPacked ? limit[MODE == kPacked ? 1 : 0][row] : 0;
+                    const int hi = MODE == kPacked ? min(limit[MODE == kPacked ? 2 : 0][row], p_end) : 0;
+#pragma unroll
+                    for (int sub = 0; sub < 2; ++sub) {
+                        const int t = t0 + 16 * sub + 4 * g4;
+                        f32x4 x = sc[rt][sub];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const int t = t0 + 16 * sub + 4 * g4 + r;
-                            const bool seen = t < va[rt] || (MODE == kPacked && t >= vlo[rt] && t < vhi[rt]);
-                            if (!(seen && t < p_end)) sc[rt][sub][r] = -INFINITY;
+                            const int hide = (int)(t + r >= va) & ((int)(t + r < lo) | (int)(t + r >= hi));
+                            x[r] = hide ? -INFINITY : x[r];
                         }
+                        sc[rt][sub] = x;
+                    }
+                }
             }
             // Scores (log2) past a row's reference by kLazy move it, for all lanes of the row.
             bool grow = false;
@@ -421,13 +495,16 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     const float mn = fmaxf(m[rt], across_max(top[rt]));
-                    const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
-                    l[rt] *= alpha;
+                    if (!first) {
+                        const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+                        l[rt] *= alpha;
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) o[rt][n] *= alpha;
+                        for (int n = 0; n < 8; ++n) o[rt][n] *= alpha;
+                    }
                     m[rt] = mn;
                 }
             }
+            first = false;
             bf16x8 pop[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -456,19 +533,22 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
             if (poison) {
                 // Rows that see a NaN value: its dimension is NaN.
                 for (int tok = 0; tok < kStep; ++tok) {
-                    const int t = t0 + tok, row = row_of[g + (tok >> 4)];
-                    if (t >= p_end || row < 0) continue;
-                    const uint32_t* src = reinterpret_cast<const uint32_t*>(P.v_cache + ((size_t)row + (tok & 15)) * D) + g4;
+                    const int t = t0 + tok, at = row_of[g + (tok >> 4)];
+                    if (t >= p_end || at < 0) continue;
+                    const uint32_t* src = reinterpret_cast<const uint32_t*>(P.v_cache + ((size_t)at + (tok & 15)) * D) + g4;
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
                         const uint32_t nb = nan_bytes(src[4 * n]);
                         if (!nb) continue;
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) {
-                            const bool seen = t < va[rt] || (MODE == kPacked && t >= vlo[rt] && t < vhi[rt]);
+                            const int row = 16 * rt + c16;
+                            int see = (int)(t < limit[0][row]);
+                            if constexpr (MODE == kPacked) see |= (int)(t >= limit[1][row]) & (int)(t < limit[2][row]);
+                            f32x4 x = o[rt][n];
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (seen && ((nb >> (8 * r)) & 1)) o[rt][n][r] = NAN;
+                            for (int r = 0; r < 4; ++r) x[r] = (see & (int)(nb >> (8 * r))) & 1 ? NAN : x[r];
+                            o[rt][n] = x;
                         }
                     }
                 }
@@ -509,7 +589,7 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
         rl += (mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - rm)) * stat[1][v][tr];
     }
     const float inv = rl == 0.f ? 0.f : 1.f / rl;
-    const int orow_h = tr / P.QT, orow_q = q0 + tr - orow_h * P.QT;
+    const int orow_h = tr * P.qt_inv >> 16, orow_q = q0 + tr - orow_h * P.QT;
     const bool live = tr < P.M && orow_q < P.Q;
     const size_t unit = ((size_t)item * P.nqt + qt) * P.Hkv + kvh;
     float es[2];
@@ -531,7 +611,7 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
             for (int v = 0; v < NW; ++v) sum[d] += ex[(size_t)(v * R + tr) * kORow + dp + d];
             sum[d] *= inv;
         }
-        if (rg.n == 1) {
+        if (n_ranges == 1) {
             if (live) {
                 uint16_t* dst = P.out + (((size_t)b * P.Q + orow_q) * P.Hq + kvh * P.G + orow_h) * D + kHalf * half + dp;
                 if constexpr (DPT % 2 == 0) {
@@ -549,8 +629,11 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
             float amax = 0.f;
 #pragma unroll
             for (int d = 0; d < DPT; ++d) amax = fmaxf(amax, fabsf(sum[d]));
-#pragma unroll
-            for (int s = 1; s < TPR; s <<= 1) amax = fmaxf(amax, __shfl_xor(amax, s, 64));
+            if constexpr (TPR >= 2) amax = fmaxf(amax, xor_asc<1>(amax));
+            if constexpr (TPR >= 4) amax = fmaxf(amax, xor_asc<2>(amax));
+            if constexpr (TPR >= 8) amax = fmaxf(amax, xor_asc<4>(amax));
+            if constexpr (TPR >= 16) amax = fmaxf(amax, xor_asc<8>(amax));
+            static_assert(TPR <= 16, "lanes of a row");
             const int e = min(max((int)((__float_as_uint(amax) >> 23) & 0xffu) - 127 - 14, -110), 110);
             es[half] = pow2(e);
             if (tr < P.M) {
@@ -560,52 +643,70 @@ __global__ __launch_bounds__(NW * 64, RT == 4 ? 1 : 2) void attn_kernel(AttnPara
             }
         }
     }
-    if (rg.n > 1 && tr < P.M && threadIdx.x % TPR == 0) P.part_ml[unit * P.M + tr] = f32x4{rm, rl, es[0], es[1]};
+    if (n_ranges > 1 && tr < P.M && threadIdx.x % TPR == 0) P.part_ml[unit * P.M + tr] = f32x4{rm, rl, es[0], es[1]};
 }
 
-// Merges the ranges of a request: workgroup (8 rows, KV head, request and
-// query tile), 32 threads per row, 4 dims each.
-constexpr int kRows = 8, kMaxRanges = 512;
-
+// Merges the ranges of a request: a wave per row, 16 lanes of 8 dims for every
+// fourth range, so that sixteen ranges' results are on the way at once.
 __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams P) {
     const int b = blockIdx.z / P.nqt, qt = blockIdx.z - b * P.nqt, kvh = blockIdx.y;
+    const int lane = threadIdx.x & 63, grp = lane >> 4, d8 = (lane & 15) * 8;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
     const Range rg = range_of_request(P, b);
-    if (rg.n == 1) return;  // written by the first launch
-    __shared__ float wt[kRows][kMaxRanges];
-    const int rr = threadIdx.x / 32, c4 = (threadIdx.x % 32) * 4, row = blockIdx.x * kRows + rr;
-    const int row_c = min(row, P.M - 1), l32 = threadIdx.x & 31;
-    const auto unit = [&](int s) { return (((size_t)(rg.first + s) * P.nqt + qt) * P.Hkv + kvh) * P.M + row_c; };
-    float mx = -INFINITY;
-    for (int s = l32; s < rg.n; s += 32) mx = fmaxf(mx, P.part_ml[unit(s)][0]);
+    const int n = __builtin_amdgcn_readfirstlane(rg.n);
+    if (n == 1) return;  // written by the first launch
+    const int gh = row * P.qt_inv >> 16, q = qt * P.QT + row - gh * P.QT;
+    if (row >= P.M || q >= P.Q) return;  // whole wave
+    const size_t u0 = (((size_t)__builtin_amdgcn_readfirstlane(rg.first) * P.nqt + qt) * P.Hkv + kvh) * P.M + row;
+    const size_t du = (size_t)P.nqt * P.Hkv * P.M;
+    float m = -INFINITY, den = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s0 = grp; s0 < n; s0 += 16) {
+        f32x4 ml[4];
+        h16x8 o[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    float den = 0.f;
-    for (int s = l32; s < rg.n; s += 32) {
-        const f32x4 ml = P.part_ml[unit(s)];
-        const float wgt = (ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mx)) * ml[1];
-        den += wgt;
-        wt[rr][s] = wgt;
-    }
+        for (int k = 0; k < 4; ++k) {
+            const size_t u = u0 + (size_t)min(s0 + 4 * k, n - 1) * du;
+            ml[k] = P.part_ml[u];
+            o[k] = *reinterpret_cast<const h16x8*>(P.part_o + u * D + d8);
+        }
+        float mn = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
-    __syncthreads();
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < rg.n; ++s) {
-        const size_t u = unit(s);
-        const float f = wt[rr][s] * P.part_ml[u][2 + (c4 >> 6)];
-        const h16x4 h = *reinterpret_cast<const h16x4*>(P.part_o + u * D + c4);
-        acc += f * f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+        for (int k = 0; k < 4; ++k) {
+            if (s0 + 4 * k >= n) ml[k] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+            mn = fmaxf(mn, ml[k][0]);
+        }
+        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        den *= keep;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[d] *= keep;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float wgt = (ml[k][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[k][0] - mn)) * ml[k][1];
+            den += wgt;
+            const float f = wgt * ml[k][2 + (d8 >> 6)];
+            if (s0 + 4 * k < n) {  // a slot past the last is not multiplied by 0: it may hold anything
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[d] = __builtin_fmaf(f, (float)o[k][d], acc[d]);
+            }
+        }
     }
+    const float mx = across_max(m);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+    den = across_sum(den * f);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) acc[d] = across_sum(acc[d] * f);
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    const int gh = row / P.QT, q = qt * P.QT + row - gh * P.QT;
-    if (row >= P.M || q >= P.Q) return;
-    *reinterpret_cast<u32x2*>(P.out + (((size_t)b * P.Q + q) * P.Hq + kvh * P.G + gh) * D + c4) =
-        u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+    if (grp == 0)
+        *reinterpret_cast<u32x4*>(P.out + (((size_t)b * P.Q + q) * P.Hq + kvh * P.G + gh) * D + d8) =
+            u32x4{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                  pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)};
 }
 
+constexpr int kMaxRanges = 512;  // of a request
+
 struct AttnPlan {
-    int QT, nqt, M, rt, items, slots, min_tiles, dense, dense_tiles;
+    int QT, nqt, M, rt, items, room, min_tiles, dense, dense_tiles;
     bool merge;
     size_t o_bytes, bytes;
 };
@@ -617,13 +718,13 @@ static AttnPlan attn_plan(int B, int Q, int Hq, int Hkv, int max_context) {
     p.nqt = (Q + p.QT - 1) / p.QT;
     p.M = G * p.QT;
     p.rt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    p.slots = p.rt == 4 ? 256 : 512;
-    p.min_tiles = 2;
+    const int slots = p.rt == 1 ? SL1 : p.rt == 2 ? SL2 : SL4;
+    p.min_tiles = p.rt == 1 ? MT1 : p.rt == 2 ? MT2 : MT4;
     const int64_t units = (int64_t)Hkv * p.nqt;
     const int tiles = (max_context + kTile - 1) / kTile;
+    p.room = (int)std::max<int64_t>(slots / units, 1);
     if (B <= 64) {
-        const int room = (int)std::max<int64_t>(p.slots / units, 1);
-        p.items = std::max(B, room);
+        p.items = std::max(B, p.room);
         const int64_t most = (int64_t)B * ((tiles + p.min_tiles - 1) / p.min_tiles);
         p.items = (int)std::min<int64_t>(p.items, std::max<int64_t>(most, 1));
         p.merge = p.items > B || (B > 1 && tiles > p.min_tiles);
@@ -682,13 +783,16 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
     P.QT = pl.QT;
     P.nqt = pl.nqt;
     P.M = pl.M;
+    P.qt_inv = (65536 + pl.QT - 1) / pl.QT;
+    P.page_shift = -1;
+    if ((page_size & (page_size - 1)) == 0) P.page_shift = __builtin_ctz((unsigned)page_size);
     P.page_size = page_size;
     P.block_shift = sh;
     P.max_pages = max_pages;
     P.num_pages = num_pages;
     P.max_context = max_context;
     P.items = pl.items;
-    P.slots = pl.slots;
+    P.room = pl.room;
     P.min_tiles = pl.min_tiles;
     P.dense = pl.dense;
     P.dense_tiles = pl.dense_tiles;
@@ -701,7 +805,7 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
         default: hipLaunchKernelGGL((attn_kernel<MODE, 4, 4>), grid, dim3(256), 0, s, P); break;
     }
     if (pl.merge)
-        hipLaunchKernelGGL(attn_merge_kernel, dim3((unsigned)((P.M + kRows - 1) / kRows), (unsigned)Hkv, (unsigned)(B * pl.nqt)),
+        hipLaunchKernelGGL(attn_merge_kernel, dim3((unsigned)((P.M + 3) / 4), (unsigned)Hkv, (unsigned)(B * pl.nqt)),
                            dim3(256), 0, s, P);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? D3D_OK : (int)err;

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -28,6 +29,7 @@ from .layers import Product, SplitProduct
 HEAD_DIM = 128
 CODE = torch.float8_e4m3fn
 SCALE = torch.float8_e8m0fnu
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 @dataclass(frozen=True, eq=False)
@@ -66,6 +68,13 @@ class Fp8KV:
             raise ValueError("a scale must cover a power of two of tokens in 16 .. 256 that divides the page size")
         if not self.num_pages or not self.kv_heads:
             raise ValueError("a cache needs at least one page and one KV head")
+        if any(t.device != self.k.device for t in (self.v, self.k_scale, self.v_scale)):
+            raise ValueError("codes and scales must be on one device")
+        # What every call passes on; the tensors live as long as this object.
+        object.__setattr__(self, "_ptrs", (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                                           self.v_scale.data_ptr()))
+        object.__setattr__(self, "_index", self.k.get_device())
+        object.__setattr__(self, "block", block)
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, kv_heads: int, device, *, block: int = 16) -> "Fp8KV":
@@ -89,10 +98,6 @@ class Fp8KV:
     def page_size(self) -> int:
         return self.k.shape[2]
 
-    @property
-    def block(self) -> int:
-        return self.k.shape[2] // self.k_scale.shape[2]
-
     def dequantize(self):
         """The values the cache stands for: bf16 (k, v) [num_pages,
         page_size, Hkv, 128], the bf16 cache's layout (exact)."""
@@ -101,17 +106,26 @@ class Fp8KV:
                      .view(P, H, ps, D).transpose(1, 2).contiguous().to(torch.bfloat16)
                      for c, s in ((self.k, self.k_scale), (self.v, self.v_scale)))
 
-    def _ptrs(self):
-        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
+
+def _check_device(cache: Fp8KV, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """The cache's HIP device, which every given tensor must be on."""
+    index = cache._index
+    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
+        _lib.require_device(cache.k, *tensors)  # raises, naming the devices
+    return cache.k.device
 
 
-def _rows(x: torch.Tensor, n: int, cache: Fp8KV, name: str) -> torch.Tensor:
-    """x as [n, Hkv, 128] bf16 whose rows are contiguous and 8-byte aligned (a
+def _rows(x: torch.Tensor, n: int, heads: int, name: str) -> torch.Tensor:
+    """x as [n, heads, 128] bf16 whose rows are contiguous and 8-byte aligned (a
     slice of a fused qkv product stays as it is)."""
-    if x.numel() != n * cache.kv_heads * HEAD_DIM:
-        raise ValueError(f"{name} must hold [tokens, {cache.kv_heads}, {HEAD_DIM}] entries")
-    x = x.reshape(n, cache.kv_heads, HEAD_DIM).to(torch.bfloat16)
-    if x.stride()[1:] != (HEAD_DIM, 1) or x.stride(0) % 4 or x.stride(0) < 0 or x.data_ptr() % 8:
+    if x.dtype is not torch.bfloat16:
+        x = x.to(torch.bfloat16)
+    if x.shape != (n, heads, HEAD_DIM):
+        if x.numel() != n * heads * HEAD_DIM:
+            raise ValueError(f"{name} must hold [tokens, {heads}, {HEAD_DIM}] entries")
+        x = x.reshape(n, heads, HEAD_DIM)
+    step, inner, one = x.stride()
+    if inner != HEAD_DIM or one != 1 or step % 4 or step < 0 or x.data_ptr() % 8:
         x = x.contiguous()
     return x
 
@@ -126,14 +140,17 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: Fp8KV, slot_mapping: torc
     too); otherwise its scale grows as the new entries need and the entries it
     holds move to it.
     """
-    dev = _lib.require_device(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, slot_mapping)
+    dev = _check_device(cache, k, v, slot_mapping)
     n = slot_mapping.numel()
-    k, v = _rows(k, n, cache, "k"), _rows(v, n, cache, "v")
-    slots = slot_mapping.reshape(n).to(torch.int64).contiguous()
-    st = _lib.load().d3d_kv_append_fp8(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), *cache._ptrs(),
-                                       slots.data_ptr(), n, cache.kv_heads, HEAD_DIM, cache.page_size, cache.block,
-                                       cache.num_pages, _lib.stream_ptr(dev))
-    _lib.check(st, "d3d_kv_append_fp8")
+    P, H, ps, _ = cache.k.shape
+    k, v = _rows(k, n, H, "k"), _rows(v, n, H, "v")
+    if slot_mapping.dtype is not torch.int64 or not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.to(torch.int64).contiguous()
+    st = _lib.load().d3d_kv_append_fp8(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), *cache._ptrs,
+                                       slot_mapping.data_ptr(), n, H, HEAD_DIM, ps, cache.block, P,
+                                       _lib.stream_ptr(dev))
+    if st:
+        _lib.check(st, "d3d_kv_append_fp8")
 
 
 def qk_rope_append(qkv: Product, positions: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
@@ -148,46 +165,52 @@ def qk_rope_append(qkv: Product, positions: torch.Tensor, q_norm: torch.Tensor, 
     """
     split = qkv if isinstance(qkv, SplitProduct) else None
     src = split.parts if split is not None else qkv
-    dev = _lib.require_device(src, positions, q_norm, k_norm, inv_freq, cache.k, cache.v, cache.k_scale,
-                              cache.v_scale, slot_mapping, q_out)
-    if heads < 1 or kv_heads != cache.kv_heads:
+    dev = _check_device(cache, src, positions, q_norm, k_norm, inv_freq, slot_mapping, q_out)
+    P, H, ps, _ = cache.k.shape
+    if heads < 1 or kv_heads != H:
         raise ValueError("the cache's KV heads do not match the model's")
     width = (heads + 2 * kv_heads) * HEAD_DIM
-    if src.dtype != (torch.bfloat16 if split is None else torch.float32) or not src.is_contiguous():
+    if src.dtype is not (torch.bfloat16 if split is None else torch.float32) or not src.is_contiguous():
         raise ValueError("qkv must be contiguous bf16 (split partials contiguous fp32)")
     if src.shape[-1] != width:
         raise ValueError("qkv row width must be (heads + 2 kv_heads) * head_dim")
     T = src.shape[1] if split is not None else src.numel() // width
     for t, name in ((positions, "positions"), (slot_mapping, "slot_mapping")):
-        if t.dtype != torch.int64 or t.numel() != T or not t.is_contiguous():
+        if t.dtype is not torch.int64 or t.numel() != T or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous int64 with one entry per token")
     for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t.dtype != torch.bfloat16 or t.numel() != HEAD_DIM or not t.is_contiguous():
+        if t.dtype is not torch.bfloat16 or t.numel() != HEAD_DIM or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous bf16 [{HEAD_DIM}]")
-    if inv_freq.dtype != torch.float32 or inv_freq.numel() != HEAD_DIM // 2 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not torch.float32 or inv_freq.numel() != HEAD_DIM // 2 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be contiguous fp32 [head_dim / 2]")
     if q_out is None:
         q_out = torch.empty(T, heads, HEAD_DIM, dtype=torch.bfloat16, device=dev)
-    elif q_out.dtype != torch.bfloat16 or q_out.numel() != T * heads * HEAD_DIM or not q_out.is_contiguous():
+    elif q_out.dtype is not torch.bfloat16 or q_out.numel() != T * heads * HEAD_DIM or not q_out.is_contiguous():
         raise ValueError("q_out must be contiguous bf16 [T, heads, head_dim]")
     tail = (positions.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
-            *cache._ptrs(), slot_mapping.data_ptr(), T, heads, kv_heads, HEAD_DIM, float(eps), cache.page_size,
-            cache.block, cache.num_pages, _lib.stream_ptr(dev))
+            *cache._ptrs, slot_mapping.data_ptr(), T, heads, kv_heads, HEAD_DIM, eps, ps, cache.block, P,
+            _lib.stream_ptr(dev))
     if split is not None:
         st = _lib.load().d3d_qk_rope_append_fp8_parts(src.data_ptr(), split.splits, *tail)
-        _lib.check(st, "d3d_qk_rope_append_fp8_parts")
     else:
         st = _lib.load().d3d_qk_rope_append_fp8(src.data_ptr(), *tail)
+    if st:
         _lib.check(st, "d3d_qk_rope_append_fp8")
     return q_out
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(B: int, Q: int, Hq: int, Hkv: int, page_size: int, max_context: int) -> int:
+    return _lib.load().d3d_attn_fp8_workspace_bytes(B, Q, Hq, Hkv, HEAD_DIM, page_size, max_context)
+
+
 def _attn(fn_name: str, q, cache: Fp8KV, lens, block_table, softmax_scale, max_seqlen_k, out, vis=None):
-    dev = _lib.require_device(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lens, block_table, vis, out)
+    dev = _check_device(cache, q, lens, block_table, vis, out)
     if q.ndim != 4:
         raise ValueError("expected q [B, Q, Hq, D]")
     B, Q, Hq, D = q.shape
-    if D != HEAD_DIM or Hq % cache.kv_heads:
+    P, H, ps, _ = cache.k.shape
+    if D != HEAD_DIM or Hq % H:
         raise ValueError("q and cache head shapes are incompatible")
     if block_table.ndim != 2 or block_table.shape[0] != B:
         raise ValueError("expected block_table [B, max_pages]")
@@ -195,26 +218,31 @@ def _attn(fn_name: str, q, cache: Fp8KV, lens, block_table, softmax_scale, max_s
         raise ValueError("expected one context length per request")
     max_pages = block_table.shape[1]
     if max_seqlen_k is None:
-        max_seqlen_k = max_pages * cache.page_size  # an upper bound that needs no host read
-    if max_seqlen_k > max_pages * cache.page_size:
-        raise ValueError("max_seqlen_k exceeds the block table's capacity")
-    q = q.to(torch.bfloat16).contiguous()
-    bt = block_table.to(torch.int32).contiguous()
-    lens = lens.to(torch.int32).reshape(B).contiguous()
+        max_seqlen_k = max_pages * ps  # an upper bound that needs no host read
+    else:
+        max_seqlen_k = int(max_seqlen_k)
+        if max_seqlen_k > max_pages * ps:
+            raise ValueError("max_seqlen_k exceeds the block table's capacity")
+    if q.dtype is not torch.bfloat16 or not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.to(torch.bfloat16).contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    if block_table.dtype is not torch.int32 or not block_table.is_contiguous():
+        block_table = block_table.to(torch.int32).contiguous()
+    if lens.dtype is not torch.int32 or not lens.is_contiguous():
+        lens = lens.to(torch.int32).contiguous()
     if out is None:
         out = torch.empty_like(q)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
+    elif out.dtype is not torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
         raise ValueError("out must be contiguous bf16 of q's shape")
-    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
-    lib = _lib.load()
-    nbytes = lib.d3d_attn_fp8_workspace_bytes(B, Q, Hq, cache.kv_heads, D, cache.page_size, int(max_seqlen_k))
-    ws = _lib.workspace(dev, "attn_fp8", nbytes)
+    ws = _lib.workspace(dev, "attn_fp8", _workspace_bytes(B, Q, Hq, H, ps, max_seqlen_k))
     vis_args = () if vis is None else (vis.data_ptr(),)
-    st = getattr(lib, fn_name)(
-        q.data_ptr(), *cache._ptrs(), bt.data_ptr(), lens.data_ptr(), *vis_args, out.data_ptr(), B, Q, Hq,
-        cache.kv_heads, D, cache.page_size, cache.block, max_pages, cache.num_pages, float(scale), int(max_seqlen_k),
+    st = getattr(_lib.load(), fn_name)(
+        q.data_ptr(), *cache._ptrs, block_table.data_ptr(), lens.data_ptr(), *vis_args, out.data_ptr(), B, Q, Hq, H, D,
+        ps, cache.block, max_pages, P, _SCALE if softmax_scale is None else softmax_scale, max_seqlen_k,
         ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
-    _lib.check(st, fn_name)
+    if st:
+        _lib.check(st, fn_name)
     return out
 
 

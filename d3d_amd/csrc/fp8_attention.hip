@@ -40,18 +40,14 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
-#ifndef SL1
-#define SL1 512
-#define SL2 512
-#define SL4 512
-#define MT1 2
-#define MT2 2
-#define MT4 2
+#ifndef DEEP
+#define DEEP 16
 #endif
 constexpr int kStep = 32;       // tokens a wave takes at a time
 constexpr int kTile = 128;      // tokens four waves take at a time: the unit of ranges
 constexpr int kMaxTiles = 64;   // tiles of a range whose pages and scales are staged at once
 constexpr int kVRow = D + 16;   // LDS bytes per value row: 16 rows, 36 banks apart, read without conflicts
+constexpr float kNone = -3.0e38f;  // the reference of a row that has seen nothing: -inf without its special cases
 constexpr float kLazy = 8.f;    // how far (log2) scores may pass the maximum that they are taken against
 
 struct AttnParams {
@@ -72,7 +68,9 @@ struct AttnParams {
     int page_size, block_shift, max_pages, num_pages;
     int max_context;
     int items;   // ranges of all requests at most
-    int room;    // ranges that run at once
+    int room;      // ranges that run at once
+    int room_one;  // the same with one workgroup per CU, where all contexts have fewer tiles than
+    int deep;
     int min_tiles;  // tiles per range at least
     int dense;   // ranges per request when items are not packed (B > 64), else 0
     int dense_tiles;
@@ -114,15 +112,19 @@ __device__ __forceinline__ int tiles_of(const AttnParams& P, int b) {
     return (max(ctx_of(P, b), 1) + kTile - 1) / kTile;
 }
 
+__device__ __forceinline__ int room_of(const AttnParams& P, int total) {
+    return total >= P.deep ? P.room : P.room_one;
+}
+
 __device__ __forceinline__ void cut_of(const AttnParams& P, int lane, int& incl, int& n) {
     const int t = lane < P.B ? tiles_of(P, lane) : 0;
-    const int total = wave_sum_int(t);
-    int tiles = max(P.min_tiles, (total + P.room - 1) / P.room);
+    const int total = wave_sum_int(t), room = room_of(P, total);
+    int tiles = max(P.min_tiles, (total + room - 1) / room);
     for (;;) {
         n = lane < P.B ? (t + tiles - 1) / tiles : 0;
         const int sum = wave_sum_int(n);
-        if (sum <= max(P.room, P.B)) break;  // one range each at the least
-        tiles += max(1, tiles * (sum - P.room) / (2 * sum));
+        if (sum <= max(room, P.B)) break;  // one range each at the least
+        tiles += max(1, tiles * (sum - room) / (2 * sum));
     }
     incl = scan_step<1>(n, lane);
     incl = scan_step<2>(incl, lane);
@@ -134,7 +136,7 @@ __device__ __forceinline__ void cut_of(const AttnParams& P, int lane, int& incl,
 
 // One request: the same, without the wave.
 __device__ __forceinline__ int cut_of_one(const AttnParams& P) {
-    const int t = tiles_of(P, 0), tiles = max(P.min_tiles, (t + P.room - 1) / P.room);
+    const int t = tiles_of(P, 0), room = room_of(P, t), tiles = max(P.min_tiles, (t + room - 1) / room);
     return (t + tiles - 1) / tiles;
 }
 
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) o[rt][n] = {0.f, 0.f, 0.f, 0.f};
-        m[rt] = -INFINITY;
+        m[rt] = kNone;
         l[rt] = 0.f;
     }
 
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
                 for (int rt = 0; rt < RT; ++rt) {
                     const float mn = fmaxf(m[rt], across_max(top[rt]));
                     if (!first) {
-                        const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+                        const float alpha = __builtin_amdgcn_exp2f(m[rt] - mn);
                         l[rt] *= alpha;
 #pragma unroll
                         for (int n = 0; n < 8; ++n) o[rt][n] *= alpha;
@@ -508,15 +510,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
             bf16x8 pop[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float off = m[rt] == -INFINITY ? 0.f : m[rt];
-                float p[8];
+                uint32_t pw[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][i >> 2][i & 3], P.scale_log2, -off));
-                    l[rt] += p[i];
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][i >> 1][2 * (i & 1)], P.scale_log2, -m[rt]));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][i >> 1][2 * (i & 1) + 1], P.scale_log2, -m[rt]));
+                    pw[i] = pack_bf16x2(p0, p1);
+                    // The sum takes the rounded probabilities, as the product does.
+                    l[rt] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw[i]), bf16x2{(__bf16)1.f, (__bf16)1.f}, l[rt], false);
                 }
-                pop[rt] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                                                           pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
+                pop[rt] = __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -569,10 +572,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     float mx[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        mx[rt] = -INFINITY;
+        mx[rt] = kNone;
 #pragma unroll
         for (int v = 0; v < NW; ++v) mx[rt] = fmaxf(mx[rt], stat[0][v][16 * rt + c16]);
-        const float f = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mx[rt]);
+        const float f = __builtin_amdgcn_exp2f(m[rt] - mx[rt]);
 #pragma unroll
         for (int n = 0; n < 8; ++n) o[rt][n] *= f;
     }
@@ -580,13 +583,12 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     constexpr int TPR = NT / R, DPT = kHalf / TPR;
     static_assert(TPR >= 1 && TPR <= 64 && DPT >= 1, "threads per row");
     const int tr = threadIdx.x / TPR, dp = (threadIdx.x % TPR) * DPT;
-    float rm = -INFINITY, rl = 0.f;
+    float rm = kNone, rl = 0.f;
 #pragma unroll
     for (int v = 0; v < NW; ++v) rm = fmaxf(rm, stat[0][v][tr]);
 #pragma unroll
     for (int v = 0; v < NW; ++v) {
-        const float mv = stat[0][v][tr];
-        rl += (mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - rm)) * stat[1][v][tr];
+        rl += __builtin_amdgcn_exp2f(stat[0][v][tr] - rm) * stat[1][v][tr];
     }
     const float inv = rl == 0.f ? 0.f : 1.f / rl;
     const int orow_h = tr * P.qt_inv >> 16, orow_q = q0 + tr - orow_h * P.QT;
@@ -646,58 +648,61 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     if (n_ranges > 1 && tr < P.M && threadIdx.x % TPR == 0) P.part_ml[unit * P.M + tr] = f32x4{rm, rl, es[0], es[1]};
 }
 
-// Merges the ranges of a request: a wave per row, 16 lanes of 8 dims for every
-// fourth range, so that sixteen ranges' results are on the way at once.
+// Merges the ranges of a request.  Sixteen lanes of 8 dims take every GR-th range
+// of a row, four of them at once: a wave per row (GR = 4) where a request has
+// many ranges, four rows per wave (GR = 1) where it has few.
+template <int GR>
 __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams P) {
     const int b = blockIdx.z / P.nqt, qt = blockIdx.z - b * P.nqt, kvh = blockIdx.y;
-    const int lane = threadIdx.x & 63, grp = lane >> 4, d8 = (lane & 15) * 8;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, grp = GR == 4 ? lane >> 4 : 0, d8 = (lane & 15) * 8;
+    const int row = GR == 4 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x * 16 + (threadIdx.x >> 4);
     const Range rg = range_of_request(P, b);
     const int n = __builtin_amdgcn_readfirstlane(rg.n);
     if (n == 1) return;  // written by the first launch
     const int gh = row * P.qt_inv >> 16, q = qt * P.QT + row - gh * P.QT;
-    if (row >= P.M || q >= P.Q) return;  // whole wave
-    const size_t u0 = (((size_t)__builtin_amdgcn_readfirstlane(rg.first) * P.nqt + qt) * P.Hkv + kvh) * P.M + row;
+    const bool live = row < P.M && q < P.Q;
+    const size_t u0 = (((size_t)__builtin_amdgcn_readfirstlane(rg.first) * P.nqt + qt) * P.Hkv + kvh) * P.M + (live ? row : 0);
     const size_t du = (size_t)P.nqt * P.Hkv * P.M;
-    float m = -INFINITY, den = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s0 = grp; s0 < n; s0 += 16) {
+    float m = kNone, den = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s0 = grp; s0 < n; s0 += 4 * GR) {
         f32x4 ml[4];
         h16x8 o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const size_t u = u0 + (size_t)min(s0 + 4 * k, n - 1) * du;
+            const size_t u = u0 + (size_t)min(s0 + GR * k, n - 1) * du;
             ml[k] = P.part_ml[u];
             o[k] = *reinterpret_cast<const h16x8*>(P.part_o + u * D + d8);
         }
         float mn = m;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (s0 + 4 * k >= n) ml[k] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+            if (s0 + GR * k >= n) ml[k] = f32x4{kNone, 0.f, 0.f, 0.f};  // the last range's again: not twice
             mn = fmaxf(mn, ml[k][0]);
         }
-        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        const float keep = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         den *= keep;
 #pragma unroll
         for (int d = 0; d < 8; ++d) acc[d] *= keep;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float wgt = (ml[k][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[k][0] - mn)) * ml[k][1];
+            const float wgt = __builtin_amdgcn_exp2f(ml[k][0] - mn) * ml[k][1];
             den += wgt;
-            const float f = wgt * ml[k][2 + (d8 >> 6)];
-            if (s0 + 4 * k < n) {  // a slot past the last is not multiplied by 0: it may hold anything
+            const float f = wgt * (d8 < 64 ? ml[k][2] : ml[k][3]);
+            if (s0 + GR * k < n) {  // a NaN that was counted already times 0
 #pragma unroll
                 for (int d = 0; d < 8; ++d) acc[d] = __builtin_fmaf(f, (float)o[k][d], acc[d]);
             }
         }
     }
-    const float mx = across_max(m);
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-    den = across_sum(den * f);
+    if constexpr (GR == 4) {
+        const float f = __builtin_amdgcn_exp2f(m - across_max(m));
+        den = across_sum(den * f);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) acc[d] = across_sum(acc[d] * f);
+        for (int d = 0; d < 8; ++d) acc[d] = across_sum(acc[d] * f);
+    }
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    if (grp == 0)
+    if (live && grp == 0)
         *reinterpret_cast<u32x4*>(P.out + (((size_t)b * P.Q + q) * P.Hq + kvh * P.G + gh) * D + d8) =
             u32x4{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
                   pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)};
@@ -706,7 +711,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams P) {
 constexpr int kMaxRanges = 512;  // of a request
 
 struct AttnPlan {
-    int QT, nqt, M, rt, items, room, min_tiles, dense, dense_tiles;
+    int QT, nqt, M, rt, items, room, room_one, deep, min_tiles, dense, dense_tiles;
     bool merge;
     size_t o_bytes, bytes;
 };
@@ -718,11 +723,16 @@ static AttnPlan attn_plan(int B, int Q, int Hq, int Hkv, int max_context) {
     p.nqt = (Q + p.QT - 1) / p.QT;
     p.M = G * p.QT;
     p.rt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    const int slots = p.rt == 1 ? SL1 : p.rt == 2 ? SL2 : SL4;
-    p.min_tiles = p.rt == 1 ? MT1 : p.rt == 2 ? MT2 : MT4;
+    // Workgroups that run at once: three per CU with one row tile, two with more.
+    // Four row tiles share a CU only from kDeep tiles per range on: a short range is
+    // mostly its own beginning and end, and more ranges mean more to merge.
     const int64_t units = (int64_t)Hkv * p.nqt;
+    const auto room = [&](int slots) { return (int)std::max<int64_t>(slots / units, 1); };
+    p.room = room(p.rt == 1 ? 768 : 512);
+    p.room_one = p.rt == 4 ? room(256) : p.room;
+    p.deep = DEEP * p.room_one;
+    p.min_tiles = p.rt == 1 ? 4 : 1;
     const int tiles = (max_context + kTile - 1) / kTile;
-    p.room = (int)std::max<int64_t>(slots / units, 1);
     if (B <= 64) {
         p.items = std::max(B, p.room);
         const int64_t most = (int64_t)B * ((tiles + p.min_tiles - 1) / p.min_tiles);
@@ -793,6 +803,8 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
     P.max_context = max_context;
     P.items = pl.items;
     P.room = pl.room;
+    P.room_one = pl.room_one;
+    P.deep = pl.deep;
     P.min_tiles = pl.min_tiles;
     P.dense = pl.dense;
     P.dense_tiles = pl.dense_tiles;
@@ -804,9 +816,13 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
         case 2: hipLaunchKernelGGL((attn_kernel<MODE, 2, 4>), grid, dim3(256), 0, s, P); break;
         default: hipLaunchKernelGGL((attn_kernel<MODE, 4, 4>), grid, dim3(256), 0, s, P); break;
     }
-    if (pl.merge)
-        hipLaunchKernelGGL(attn_merge_kernel, dim3((unsigned)((P.M + 3) / 4), (unsigned)Hkv, (unsigned)(B * pl.nqt)),
-                           dim3(256), 0, s, P);
+    if (pl.merge) {
+        const unsigned y = (unsigned)Hkv, z = (unsigned)(B * pl.nqt);
+        if (pl.items > 4 * B)
+            hipLaunchKernelGGL((attn_merge_kernel<4>), dim3((unsigned)((P.M + 3) / 4), y, z), dim3(256), 0, s, P);
+        else
+            hipLaunchKernelGGL((attn_merge_kernel<1>), dim3((unsigned)((P.M + 15) / 16), y, z), dim3(256), 0, s, P);
+    }
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? D3D_OK : (int)err;
 }

@@ -234,32 +234,51 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     const int n_ranges = __builtin_amdgcn_readfirstlane(rg.n);
     const int len = __builtin_amdgcn_readfirstlane(min(P.context_lens[b], P.max_pages * P.page_size));
     const int ctx = min(len, P.max_context), pre = len - P.Q, q0 = qt * P.QT;
-    // The request's tiles in n_ranges even parts.
-    const uint64_t tiles = (uint64_t)((max(ctx, 1) + kTile - 1) / kTile), s_r = (uint64_t)__builtin_amdgcn_readfirstlane(rg.s);
-    const int t_begin = (int)(s_r * tiles / n_ranges) * kTile;
-    const int t_last = min((int)((s_r + 1) * tiles / n_ranges) * kTile, ctx);
+    // The request's tiles in n_ranges even parts, the first ones a tile longer.
+    const int tiles = (max(ctx, 1) + kTile - 1) / kTile, s_r = __builtin_amdgcn_readfirstlane(rg.s);
+    const int part = tiles / n_ranges, longer = tiles - part * n_ranges;
+    const int t_begin = (s_r * part + min(s_r, longer)) * kTile;
+    const int t_last = min(t_begin + (part + (s_r < longer ? 1 : 0)) * kTile, ctx);
 
-    // This lane's rows: head gh of the group, query qi.  The frontier goes by the
-    // context's own length, reads by its bounds.
+    // The page of a 16-token group of the piece from p0 on; -1 behind its end.
+    const auto page_at = [&](int p0, int i) {
+        const int t = p0 + 16 * i;
+        if (i >= kGroups || t >= t_last) return -1;
+        return P.block_table[(size_t)b * P.max_pages + (P.page_shift >= 0 ? t >> P.page_shift : t / P.page_size)];
+    };
+    int page = page_at(t_begin, threadIdx.x);  // on its way beside the queries
+
+    // Q^T operands: dims 64 p + 16 g4 + 8 e .. + 7 at ks = 2 p + e, as the keys are
+    // loaded.  Rows behind the last are a copy of row 0 that nobody writes out.
+    const uint16_t* q_rows = P.q + ((size_t)b * P.Q * P.Hq + (size_t)kvh * P.G) * D + 16 * g4;
+    const auto load_q = [&](int row, int ks) {
+        const int gh = row * P.qt_inv >> 16, qi = q0 + row - gh * P.QT;
+        const size_t at = row < P.M && qi < P.Q ? (size_t)qi * P.Hq + gh : 0;
+        return *reinterpret_cast<const u32x4*>(q_rows + at * D + 64 * (ks >> 1) + 8 * (ks & 1));
+    };
     bf16x8 qop[QLDS ? 1 : RT][4];
-    int a_min = INT_MAX, a_max = 0, s_lo = INT_MAX, s_hi = 0;
+    if constexpr (QLDS) {
+        static_assert(!QLDS || RT == NW, "a row tile per wave");
+        u32x4 v[4];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = rt * 16 + c16, gh = row * P.qt_inv >> 16, qi = q0 + row - gh * P.QT;
-        const bool row_ok = row < P.M && qi < P.Q;
-        // Q^T operands: dims 64 p + 16 g4 + 8 e .. + 7 at ks = 2 p + e, as the keys are loaded.
-        if (!QLDS || rt % NW == w) {
-            const uint16_t* src = P.q + (((size_t)b * P.Q + (row_ok ? qi : 0)) * P.Hq + kvh * P.G + (row_ok ? gh : 0)) * D + 16 * g4;
+        for (int ks = 0; ks < 4; ++ks) v[ks] = load_q(16 * w + c16, ks);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                u32x4 v = *reinterpret_cast<const u32x4*>(src + 64 * (ks >> 1) + 8 * (ks & 1));
-                if (!row_ok) v = u32x4{0u, 0u, 0u, 0u};
-                if constexpr (QLDS)
-                    *reinterpret_cast<u32x4*>(lds + kVBytes + ((rt * 4 + ks) * 64 + lane) * 16) = v;
-                else
-                    qop[rt][ks] = __builtin_bit_cast(bf16x8, v);
-            }
-        }
+        for (int ks = 0; ks < 4; ++ks) *reinterpret_cast<u32x4*>(lds + kVBytes + ((w * 4 + ks) * 64 + lane) * 16) = v[ks];
+    } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) qop[rt][ks] = __builtin_bit_cast(bf16x8, load_q(16 * rt + c16, ks));
+    }
+
+    // The rows' limits, a row per lane, kept in LDS: they are read where a step has
+    // keys that some row does not see.  The frontier goes by the context's own
+    // length, reads by its bounds.  Over all rows: keys below a_min are seen by
+    // each, none from a_max on by any but [s_lo, s_hi).
+    int a_min, a_max, s_lo = 0, s_hi = 0;
+    {
+        const int gh = lane * P.qt_inv >> 16, qi = q0 + lane - gh * P.QT;
+        const bool row_ok = lane < P.M && qi < P.Q;
         int va = 0, lo = 0, hi = 0;
         if (row_ok) {
             va = ctx;
@@ -268,43 +287,34 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
                 va = min(pre + P.vis[qi * 3], ctx);
                 lo = max(pre + P.vis[qi * 3 + 1], 0);
                 hi = min(pre + P.vis[qi * 3 + 2], ctx);
-                a_min = min(a_min, va);
-                a_max = max(a_max, va);
-                if (lo < hi) {
-                    s_lo = min(s_lo, lo);
-                    s_hi = max(s_hi, hi);
-                }
             }
         }
-        // Every wave has the same rows; they are read where a step has keys that
-        // some row does not see, which leaves the registers to the main loop.
-        if (g4 == 0 && w == 0) {
-            limit[0][row] = va;
+        if (w == 0 && lane < R) {
+            limit[0][lane] = va;
             if constexpr (MODE == kPacked) {
-                limit[1][row] = lo;
-                limit[2][row] = hi;
+                limit[1][lane] = lo;
+                limit[2][lane] = hi;
             }
         }
-    }
-    // Over all rows: keys below a_min are seen by each, none from a_max on by any but [s_lo, s_hi).
-    if constexpr (MODE == kPacked) {
-        const auto all = [](int& v, auto f) {
-            v = f(v, xor_desc<8>(v));
-            v = f(v, xor_desc<4>(v));
-            v = f(v, xor_desc<2>(v));
-            v = __builtin_amdgcn_readfirstlane(f(v, xor_desc<1>(v)));
-        };
-        const auto lo = [](int x, int y) { return min(x, y); };
-        const auto hi = [](int x, int y) { return max(x, y); };
-        all(a_min, lo);
-        all(a_max, hi);
-        all(s_lo, lo);
-        all(s_hi, hi);
-    } else if constexpr (MODE == kCausal) {
-        a_min = min(pre + q0 + 1, ctx);
-        a_max = min(pre + min(q0 + P.QT, P.Q), ctx);
-    } else {
-        a_min = a_max = ctx;
+        if constexpr (MODE == kPacked) {
+            const auto largest = [](int v) {
+                v = max(v, xor_desc<32>(v));
+                v = max(v, xor_desc<16>(v));
+                v = max(v, xor_desc<8>(v));
+                v = max(v, xor_desc<4>(v));
+                v = max(v, xor_desc<2>(v));
+                return __builtin_amdgcn_readfirstlane(max(v, xor_desc<1>(v)));
+            };
+            a_min = -largest(row_ok ? -va : -INT_MAX);
+            a_max = largest(va);
+            s_lo = -largest(lo < hi ? -lo : -INT_MAX);
+            s_hi = largest(lo < hi ? hi : 0);
+        } else if constexpr (MODE == kCausal) {
+            a_min = min(pre + q0 + 1, ctx);
+            a_max = min(pre + min(q0 + P.QT, P.Q), ctx);
+        } else {
+            a_min = a_max = ctx;
+        }
     }
 
     f32x4 o[RT][8];
@@ -343,24 +353,31 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
         const auto step_at = [&](int j) { return j < n1 ? j : st2 + j - n1; };
         __syncthreads();  // the tables of the piece before are no longer read
         const int groups = 2 * (step_at(steps - 1) + 1);
-        constexpr int kPer = kGroups / NT;
-        int row[kPer];
-        size_t at[kPer];
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int i = threadIdx.x + k * NT, t = p0 + 16 * i;
-            row[k] = -1;
-            at[k] = 0;
-            if (i < groups && t < p_end) {
-                const int pi = P.page_shift >= 0 ? t >> P.page_shift : t / P.page_size, in = t - pi * P.page_size;
-                const int page = P.block_table[(size_t)b * P.max_pages + pi];
-                if (page >= 0 && page < P.num_pages) {
-                    const size_t ph = (size_t)page * P.Hkv + kvh;
-                    at[k] = ph * (P.page_size >> P.block_shift) + (in >> P.block_shift);
-                    row[k] = (int)(ph * P.page_size + in);
-                }
+        if (p0 != t_begin) page = page_at(p0, threadIdx.x);
+        // A group's first row, and the place of its scales.
+        const auto place = [&](int i, int pg, size_t& at) {
+            int row = -1;
+            at = 0;
+            if (pg >= 0 && pg < P.num_pages) {
+                const int t = p0 + 16 * i, in = P.page_shift >= 0 ? t & (P.page_size - 1) : t % P.page_size;
+                const size_t ph = (size_t)pg * P.Hkv + kvh;
+                at = ph * (P.page_size >> P.block_shift) + (in >> P.block_shift);
+                row = (int)(ph * P.page_size + in);
             }
-            if (i < groups) row_of[i] = row[k];
+            row_of[i] = row;
+            return row;
+        };
+        const auto put_scale = [&](int i, int row, size_t at) {
+            scale_of[i] = row < 0 ? u32x2{0x3f800000u, 0x3f800000u}
+                                  : u32x2{(uint32_t)P.k_scale[at] << 23, (uint32_t)P.v_scale[at] << 23};
+        };
+        size_t at;
+        const int first_row = place(threadIdx.x, page, at);
+        static_assert(kGroups == 2 * NT, "groups per thread");
+        if (groups > NT) {  // uniform
+            size_t at2;
+            const int row2 = place(threadIdx.x + NT, page_at(p0, threadIdx.x + NT), at2);
+            put_scale(threadIdx.x + NT, row2, at2);
         }
         __syncthreads();
 
@@ -386,14 +403,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
             fetch_k(w);
             fetch_v(w);
         }
-        // The scales come beside the first keys and values.
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int i = threadIdx.x + k * NT;
-            if (i < groups)
-                scale_of[i] = row[k] < 0 ? u32x2{0x3f800000u, 0x3f800000u}
-                                         : u32x2{(uint32_t)P.k_scale[at[k]] << 23, (uint32_t)P.v_scale[at[k]] << 23};
-        }
+        put_scale(threadIdx.x, first_row, at);  // beside the first keys and values
         __syncthreads();
         for (int j = w; j < steps; j += NW) {
             const int t0 = p0 + kStep * step_at(j), g = 2 * step_at(j);
@@ -569,28 +579,21 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
         }
     }
     __syncthreads();  // also: no wave reads its value rows any more
-    float mx[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        mx[rt] = kNone;
-#pragma unroll
-        for (int v = 0; v < NW; ++v) mx[rt] = fmaxf(mx[rt], stat[0][v][16 * rt + c16]);
-        const float f = __builtin_amdgcn_exp2f(m[rt] - mx[rt]);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) o[rt][n] *= f;
-    }
     // Thread tid adds up dims dp .. of row tr; TPR threads per row.
     constexpr int TPR = NT / R, DPT = kHalf / TPR;
     static_assert(TPR >= 1 && TPR <= 64 && DPT >= 1, "threads per row");
     const int tr = threadIdx.x / TPR, dp = (threadIdx.x % TPR) * DPT;
-    float rm = kNone, rl = 0.f;
+    float rm = kNone, rl = 0.f, fv[NW];
 #pragma unroll
     for (int v = 0; v < NW; ++v) rm = fmaxf(rm, stat[0][v][tr]);
 #pragma unroll
     for (int v = 0; v < NW; ++v) {
-        rl += __builtin_amdgcn_exp2f(stat[0][v][tr] - rm) * stat[1][v][tr];
+        fv[v] = __builtin_amdgcn_exp2f(stat[0][v][tr] - rm);
+        rl = __builtin_fmaf(fv[v], stat[1][v][tr], rl);
     }
     const float inv = rl == 0.f ? 0.f : 1.f / rl;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) fv[v] *= inv;
     const int orow_h = tr * P.qt_inv >> 16, orow_q = q0 + tr - orow_h * P.QT;
     const bool live = tr < P.M && orow_q < P.Q;
     const size_t unit = ((size_t)item * P.nqt + qt) * P.Hkv + kvh;
@@ -603,15 +606,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
-                *reinterpret_cast<f32x4*>(ex + (size_t)(w * R + 16 * rt + c16) * kORow + 16 * n + 4 * g4) = o[rt][4 * half + n];
+                *reinterpret_cast<f32x4*>(ex + (w * R + 16 * rt + c16) * kORow + 16 * n + 4 * g4) = o[rt][4 * half + n];
         __syncthreads();
         float sum[DPT];
 #pragma unroll
         for (int d = 0; d < DPT; ++d) {
             sum[d] = 0.f;
 #pragma unroll
-            for (int v = 0; v < NW; ++v) sum[d] += ex[(size_t)(v * R + tr) * kORow + dp + d];
-            sum[d] *= inv;
+            for (int v = 0; v < NW; ++v) sum[d] = __builtin_fmaf(fv[v], ex[(v * R + tr) * kORow + dp + d], sum[d]);
         }
         if (n_ranges == 1) {
             if (live) {

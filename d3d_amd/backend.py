@@ -5,7 +5,8 @@ Mirrors serving/backend.py:
 * ``Runner(path, device, *, draft=False, pages=512)`` -- :24-53: one model
   (target or draft) with its paged K/V cache and page pool on one device;
   ``path`` names a model shape (there is no checkpoint loading: weights are
-  random-initialised bf16), see :func:`resolve_shape`;
+  random-initialised bf16), see :func:`resolve_shape`; ``kv_dtype="fp8"``
+  keeps keys and values in 8 bits (see model.PagedKV);
 * ``reserve`` / ``release`` / ``trim`` / ``_tables`` -- :55-76, the page
   bookkeeping (device-resident tables here, see model.DevicePageTables);
 * ``prefill(seqs)`` -- :98-112: the prompts' K/V and the greedy token after
@@ -94,7 +95,7 @@ class SamplingParams:
 
 class Runner:
     def __init__(self, path, device="cuda:0", *, draft: bool = False, pages: int = 512, page_size: int = 16,
-                 seed: Optional[int] = None, use_graphs: bool = True):
+                 seed: Optional[int] = None, use_graphs: bool = True, kv_dtype: str = "bf16"):
         self.device = torch.device(device)
         self.draft = draft
         shape = resolve_shape(path)
@@ -108,7 +109,7 @@ class Runner:
         num_pages = max(1, pages * PAGE // page_size)
         self.model = Qwen3PagedModel(shape, self.device, draft=draft, seed=(1 if draft else 0) if seed is None
                                      else seed)
-        self.kv = PagedKV(shape, num_pages, page_size, self.device)
+        self.kv = PagedKV(shape, num_pages, page_size, self.device, kv_dtype=kv_dtype)
         self.pool = self.kv.pool
         self.stream = dedicated_stream(self.device, "draft" if draft else "target")
         self.use_graphs = use_graphs

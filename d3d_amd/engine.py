@@ -19,9 +19,11 @@ same constructor, methods and result dictionary:
   release and the leak checks.
 
 Keywords past the reference's (``device``, ``page_size``, ``mask_id``,
-``use_graphs``, ``tuned_gemms``) choose the device, the KV page size, the
-draft's mask id, whether steps replay HIP graphs, and whether the step's
-library GEMMs use the solution choices in gemm_tuned_gfx950.csv
+``use_graphs``, ``tuned_gemms``, ``kv_dtype``) choose the device, the KV page
+size, the draft's mask id, whether steps replay HIP graphs, whether both
+models' keys and values are kept in 8 bits (``kv_dtype="fp8"``: half the bytes,
+see fp8_kv; what a block is verified against then depends in the last bits
+on the blocks rejected before it), and whether the step's library GEMMs use the solution choices in gemm_tuned_gfx950.csv
 (``tuned_gemms=True``, off by default: gemm_tuning.enable turns on
 TunableOp, a process-wide torch switch, and ``close()`` turns it back; a
 no-op where the file's library versions or GPU do not match).
@@ -133,7 +135,8 @@ class Engine:
     def __init__(self, target, draft, block_size: int = 16, anchor_num: int = 3, draft_microbatch: int = 4,
                  pages: int = 512, backup: str = "neural", seed: int = 42, fast_miss_anchors: int = 0,
                  draft_pages: Optional[int] = None, *, device: str = "cuda:0", page_size: int = 16,
-                 mask_id: int = MASK_ID, use_graphs: bool = True, tuned_gemms: bool = False):
+                 mask_id: int = MASK_ID, use_graphs: bool = True, tuned_gemms: bool = False,
+                 kv_dtype: str = "bf16"):
         if backup not in ("neural", "fast", "fast_legacy"):
             raise ValueError(backup)
         if anchor_num < 1:
@@ -159,9 +162,9 @@ class Engine:
         self._tunable_saved = gemm_tuning.state() if tuned_gemms else None
         self.tuned_gemms = gemm_tuning.enable() if tuned_gemms else False
         self.target = Runner(target, self.device, pages=pages, page_size=page_size, seed=seed,
-                             use_graphs=use_graphs)
+                             use_graphs=use_graphs, kv_dtype=kv_dtype)
         self.draft = Runner(draft, self.device, draft=True, pages=pages if draft_pages is None else draft_pages,
-                            page_size=page_size, seed=seed + 1, use_graphs=use_graphs)
+                            page_size=page_size, seed=seed + 1, use_graphs=use_graphs, kv_dtype=kv_dtype)
         if self.target.shape.vocab != self.draft.shape.vocab:
             raise ValueError("target and draft vocabularies must match")
         if not 0 <= mask_id < self.draft.shape.vocab:

@@ -39,6 +39,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import attention as att
+from . import fp8_kv
 from . import layers as ly
 
 
@@ -163,14 +164,30 @@ class DevicePageTables:
 
 
 class PagedKV:
-    """Per-layer K/V caches [num_pages, page_size, Hkv, D] bf16 (serving/backend.py:46-48)."""
+    """Per-layer K/V caches of one model and their page pool.
 
-    def __init__(self, shape: ModelShape, num_pages: int, page_size: int, device):
+    ``kv_dtype="bf16"``: ``k``, ``v`` [num_pages, page_size, Hkv, D] per layer
+    (serving/backend.py:46-48).  ``kv_dtype="fp8"``: ``fp8``, an 8-bit cache
+    (:class:`d3d_amd.fp8_kv.Fp8KV`) per layer with a scale for ``scale_block``
+    tokens, half the bytes; ``k`` and ``v`` are empty then."""
+
+    def __init__(self, shape: ModelShape, num_pages: int, page_size: int, device, *, kv_dtype: str = "bf16",
+                 scale_block: int = 16):
+        if kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r}: bf16 or fp8")
         self.page_size = page_size
         self.num_pages = num_pages
-        self.k = [torch.zeros(num_pages, page_size, shape.kv_heads, shape.head_dim, dtype=torch.bfloat16,
-                              device=device) for _ in range(shape.layers)]
-        self.v = [torch.zeros_like(t) for t in self.k]
+        self.kv_dtype = kv_dtype
+        self.k, self.v, self.fp8 = [], [], []
+        if kv_dtype == "fp8":
+            if shape.head_dim != fp8_kv.HEAD_DIM:
+                raise ValueError(f"the 8-bit cache takes a head dimension of {fp8_kv.HEAD_DIM}")
+            self.fp8 = [fp8_kv.Fp8KV.empty(num_pages, page_size, shape.kv_heads, device, block=scale_block)
+                        for _ in range(shape.layers)]
+        else:
+            self.k = [torch.zeros(num_pages, page_size, shape.kv_heads, shape.head_dim, dtype=torch.bfloat16,
+                                  device=device) for _ in range(shape.layers)]
+            self.v = [torch.zeros_like(t) for t in self.k]
         self.pool = PagePool(num_pages)
         self.tables = DevicePageTables(num_pages, device)
 
@@ -219,6 +236,8 @@ class Qwen3PagedModel(torch.nn.Module):
         add + RMSNorm, QKV GEMM, fused q/k norm + RoPE + KV append, paged
         attention, O GEMM, fused add + RMSNorm, gate-up GEMM, fused SiLU-mul,
         down GEMM (the decoder layer of serving/vendor/ssd/models/qwen3.py).
+        Over an 8-bit cache (``kv.fp8``) the append quantises and the attention
+        reads the codes; norm and rotation then run in fp32 for both models.
         Blocks of at most 192 tokens run the projections on the
         weight-streaming HIP GEMM where layers.project / gate_up_silu pick it
         (when ``rows64_gemm``: the QKV, O and down GEMMs, whose K-split
@@ -240,14 +259,25 @@ class Qwen3PagedModel(torch.nn.Module):
             if li:
                 ly.add_rmsnorm(x, residual, L["ln1"], s.eps, out=hs)
             qkv = proj(hs, L["qkv"])
-            q = ly.qk_rope_append(qkv, pos, L["qn"], L["kn"], self.inv_freq, kv.k[li], kv.v[li], slot_mapping,
-                                  Hq, Hkv, s.eps, draft_rope=self.draft)
-            if q_vis is None:
-                o = att.flash_attn_with_kvcache(q.view(B, Q, Hq, d), kv.k[li], kv.v[li], context_lens,
-                                                block_tables, causal=causal, max_seqlen_k=max_context)
+            if kv.fp8:
+                cache = kv.fp8[li]
+                q = fp8_kv.qk_rope_append(qkv, pos, L["qn"], L["kn"], self.inv_freq, cache, slot_mapping, Hq, Hkv,
+                                          s.eps).view(B, Q, Hq, d)
+                if q_vis is None:
+                    o = fp8_kv.flash_attn_with_kvcache(q, cache, context_lens, block_tables, causal=causal,
+                                                       max_seqlen_k=max_context)
+                else:
+                    o = fp8_kv.packed_block_attn(q, cache, context_lens, block_tables, q_vis,
+                                                 max_seqlen_k=max_context)
             else:
-                o = att.packed_block_attn(q.view(B, Q, Hq, d), kv.k[li], kv.v[li], context_lens, block_tables,
-                                          q_vis, max_seqlen_k=max_context)
+                q = ly.qk_rope_append(qkv, pos, L["qn"], L["kn"], self.inv_freq, kv.k[li], kv.v[li], slot_mapping,
+                                      Hq, Hkv, s.eps, draft_rope=self.draft)
+                if q_vis is None:
+                    o = att.flash_attn_with_kvcache(q.view(B, Q, Hq, d), kv.k[li], kv.v[li], context_lens,
+                                                    block_tables, causal=causal, max_seqlen_k=max_context)
+                else:
+                    o = att.packed_block_attn(q.view(B, Q, Hq, d), kv.k[li], kv.v[li], context_lens, block_tables,
+                                              q_vis, max_seqlen_k=max_context)
             x = proj(o.reshape(B * Q, Hq * d), L["o"])
             ly.add_rmsnorm(x, residual, L["ln2"], s.eps, out=hs)
             act = ly.gate_up_silu(hs, L["gate_up"]) if self.rows64_gemm else ly.silu_mul(F.linear(hs, L["gate_up"]))

@@ -114,18 +114,21 @@ class D3DForCausalLM:
 
     ``shape`` defaults to the D3D-1.7B draft (28 layers, hidden 2048, 16/8
     heads, MLP 6144, V 151,936); ``pages`` x ``page_size`` tokens of K/V
-    are shared by every PagedCache of this model.
+    (``kv_dtype`` "bf16", or "fp8" for the 8-bit cache) are shared by every
+    PagedCache of this model.
     """
 
     name = "draft"
 
     def __init__(self, shape: ModelShape = D3D_1P7B, device="cuda:0", *, pages: int = 4096, page_size: int = 16,
-                 seed: int = 0, model: Optional[Qwen3PagedModel] = None, kv: Optional[PagedKV] = None):
+                 seed: int = 0, model: Optional[Qwen3PagedModel] = None, kv: Optional[PagedKV] = None,
+                 kv_dtype: str = "bf16"):
         self.device = torch.device(device)
         self.model = model if model is not None else Qwen3PagedModel(shape, self.device, draft=True, seed=seed)
         self.config = SimpleNamespace(vocab_size=self.model.shape.vocab, num_hidden_layers=self.model.shape.layers,
                                       hidden_size=self.model.shape.hidden)
-        self.kv = kv if kv is not None else PagedKV(self.model.shape, pages, page_size, self.device)
+        self.kv = kv if kv is not None else PagedKV(self.model.shape, pages, page_size, self.device,
+                                                    kv_dtype=kv_dtype)
         self._next_id = 0
 
     def _new_sequence(self) -> Sequence:

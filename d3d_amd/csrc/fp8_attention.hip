@@ -40,11 +40,13 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
-#ifndef DEEP
-#define DEEP 16
-#endif
 constexpr int kStep = 32;       // tokens a wave takes at a time
 constexpr int kTile = 128;      // tokens four waves take at a time: the unit of ranges
+// Tiles per range from which four row tiles take two workgroups per CU: a short
+// range is mostly its own beginning and end, and more ranges mean more to merge
+// (8 requests of 608 to 2,432 tokens and 16 rows: 17.0 + 5.0 us with one, 19.1
+// + 5.5 with two; two of 131,072 tokens: 105 with one, 103 with two).
+constexpr int kDeep = 16;
 constexpr int kMaxTiles = 64;   // tiles of a range whose pages and scales are staged at once
 constexpr int kVRow = D + 16;   // LDS bytes per value row: 16 rows, 36 banks apart, read without conflicts
 constexpr float kNone = -3.0e38f;  // the reference of a row that has seen nothing: -inf without its special cases
@@ -69,8 +71,8 @@ struct AttnParams {
     int max_context;
     int items;   // ranges of all requests at most
     int room;      // ranges that run at once
-    int room_one;  // the same with one workgroup per CU, where all contexts have fewer tiles than
-    int deep;
+    int room_one;  // the same with one workgroup per CU,
+    int deep;      // where all contexts together have fewer tiles than this
     int min_tiles;  // tiles per range at least
     int dense;   // ranges per request when items are not packed (B > 64), else 0
     int dense_tiles;
@@ -102,7 +104,7 @@ __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_am
 
 // How the contexts are cut, the same in every workgroup of both launches.  Up
 // to 64 requests: with the least number of tiles per range that keeps the
-// ranges of all requests within P.slots workgroups; item numbers run through
+// ranges of all requests within P.room workgroups; item numbers run through
 // the requests' own range counts.  A whole wave calls it.
 struct Range {
     int b, s, n, first;  // request (-1: none), range, ranges of the request, its first item
@@ -124,7 +126,7 @@ __device__ __forceinline__ void cut_of(const AttnParams& P, int lane, int& incl,
         n = lane < P.B ? (t + tiles - 1) / tiles : 0;
         const int sum = wave_sum_int(n);
         if (sum <= max(room, P.B)) break;  // one range each at the least
-        tiles += max(1, tiles * (sum - room) / (2 * sum));
+        tiles += max(1, (int)((float)tiles * (float)(sum - room) / (float)(2 * sum)));
     }
     incl = scan_step<1>(n, lane);
     incl = scan_step<2>(incl, lane);
@@ -726,13 +728,11 @@ static AttnPlan attn_plan(int B, int Q, int Hq, int Hkv, int max_context) {
     p.M = G * p.QT;
     p.rt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
     // Workgroups that run at once: three per CU with one row tile, two with more.
-    // Four row tiles share a CU only from kDeep tiles per range on: a short range is
-    // mostly its own beginning and end, and more ranges mean more to merge.
     const int64_t units = (int64_t)Hkv * p.nqt;
     const auto room = [&](int slots) { return (int)std::max<int64_t>(slots / units, 1); };
     p.room = room(p.rt == 1 ? 768 : 512);
     p.room_one = p.rt == 4 ? room(256) : p.room;
-    p.deep = DEEP * p.room_one;
+    p.deep = kDeep * p.room_one;
     p.min_tiles = p.rt == 1 ? 4 : 1;
     const int tiles = (max_context + kTile - 1) / kTile;
     if (B <= 64) {
@@ -768,6 +768,7 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
     if ((int64_t)num_pages * page_size > INT_MAX / Hkv) return D3D_E_SHAPE;  // rows of a cache
     const int sh = fp8_block_shift(page_size, block);
     if (sh < 0) return D3D_E_UNSUPPORTED;
+    if (!(scale > 0.f && scale < INFINITY)) return D3D_E_UNSUPPORTED;  // a masked score is -inf times it
     if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !context_lens || !out) return D3D_E_NULL;
     if (MODE == kPacked && !vis) return D3D_E_NULL;
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16)
@@ -835,7 +836,8 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
 using namespace d3d;
 
 extern "C" size_t d3d_attn_fp8_workspace_bytes(int B, int Q, int Hq, int Hkv, int D, int page_size, int max_context) {
-    if (B < 1 || Q < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || D != fp8::D || page_size < 1 || max_context < 1 || Hq / Hkv > 64)
+    if (B < 1 || Q < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || D != fp8::D || page_size < 1 || max_context < 1 ||
+        max_context > INT_MAX / 2 || Hq / Hkv > 64)
         return 0;
     return fp8::attn_plan(B, Q, Hq, Hkv, max_context).bytes;
 }

@@ -70,9 +70,6 @@ class Fp8KV:
             raise ValueError("a cache needs at least one page and one KV head")
         if any(t.device != self.k.device for t in (self.v, self.k_scale, self.v_scale)):
             raise ValueError("codes and scales must be on one device")
-        # What every call passes on; the tensors live as long as this object.
-        object.__setattr__(self, "_ptrs", (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
-                                           self.v_scale.data_ptr()))
         object.__setattr__(self, "_index", self.k.get_device())
         object.__setattr__(self, "block", block)
 
@@ -97,6 +94,9 @@ class Fp8KV:
     @property
     def page_size(self) -> int:
         return self.k.shape[2]
+
+    def _ptrs(self):
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     def dequantize(self):
         """The values the cache stands for: bf16 (k, v) [num_pages,
@@ -125,8 +125,8 @@ def _rows(x: torch.Tensor, n: int, heads: int, name: str) -> torch.Tensor:
             raise ValueError(f"{name} must hold [tokens, {heads}, {HEAD_DIM}] entries")
         x = x.reshape(n, heads, HEAD_DIM)
     step, inner, one = x.stride()
-    if inner != HEAD_DIM or one != 1 or step % 4 or step < 0 or x.data_ptr() % 8:
-        x = x.contiguous()
+    if inner != HEAD_DIM or one != 1 or step % 4 or x.data_ptr() % 8:
+        x = x.clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd address, or one row's stride
     return x
 
 
@@ -146,7 +146,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: Fp8KV, slot_mapping: torc
     k, v = _rows(k, n, H, "k"), _rows(v, n, H, "v")
     if slot_mapping.dtype is not torch.int64 or not slot_mapping.is_contiguous():
         slot_mapping = slot_mapping.to(torch.int64).contiguous()
-    st = _lib.load().d3d_kv_append_fp8(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), *cache._ptrs,
+    st = _lib.load().d3d_kv_append_fp8(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), *cache._ptrs(),
                                        slot_mapping.data_ptr(), n, H, HEAD_DIM, ps, cache.block, P,
                                        _lib.stream_ptr(dev))
     if st:
@@ -160,8 +160,9 @@ def qk_rope_append(qkv: Product, positions: torch.Tensor, q_norm: torch.Tensor, 
 
     ``qkv`` [T, (Hq + 2 Hkv) * 128] bf16, or a SplitProduct of
     ``layers.project``; ``positions`` and ``slot_mapping`` [T] int64.  Norm and
-    rotation run in fp32 with one rounding at the end (q to bf16, k to its
-    code), for the target and the draft alike; the store is ``kv_append``'s.
+    rotation run in fp32 for q, with one rounding to bf16 at the end, and in
+    64 bits for k, whose result is rounded to its code, for the target and the
+    draft alike; the store is ``kv_append``'s.
     """
     split = qkv if isinstance(qkv, SplitProduct) else None
     src = split.parts if split is not None else qkv
@@ -188,7 +189,7 @@ def qk_rope_append(qkv: Product, positions: torch.Tensor, q_norm: torch.Tensor, 
     elif q_out.dtype is not torch.bfloat16 or q_out.numel() != T * heads * HEAD_DIM or not q_out.is_contiguous():
         raise ValueError("q_out must be contiguous bf16 [T, heads, head_dim]")
     tail = (positions.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
-            *cache._ptrs, slot_mapping.data_ptr(), T, heads, kv_heads, HEAD_DIM, eps, ps, cache.block, P,
+            *cache._ptrs(), slot_mapping.data_ptr(), T, heads, kv_heads, HEAD_DIM, eps, ps, cache.block, P,
             _lib.stream_ptr(dev))
     if split is not None:
         st = _lib.load().d3d_qk_rope_append_fp8_parts(src.data_ptr(), split.splits, *tail)
@@ -238,7 +239,7 @@ def _attn(fn_name: str, q, cache: Fp8KV, lens, block_table, softmax_scale, max_s
     ws = _lib.workspace(dev, "attn_fp8", _workspace_bytes(B, Q, Hq, H, ps, max_seqlen_k))
     vis_args = () if vis is None else (vis.data_ptr(),)
     st = getattr(_lib.load(), fn_name)(
-        q.data_ptr(), *cache._ptrs, block_table.data_ptr(), lens.data_ptr(), *vis_args, out.data_ptr(), B, Q, Hq, H, D,
+        q.data_ptr(), *cache._ptrs(), block_table.data_ptr(), lens.data_ptr(), *vis_args, out.data_ptr(), B, Q, Hq, H, D,
         ps, cache.block, max_pages, P, _SCALE if softmax_scale is None else softmax_scale, max_seqlen_k,
         ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
     if st:
@@ -254,7 +255,8 @@ def flash_attn_with_kvcache(q: torch.Tensor, cache: Fp8KV, cache_seqlens: torch.
     With ``causal=True`` query i sees keys j <= cache_seqlens[b] - Q + i; with
     ``causal=False`` every key j < cache_seqlens[b].  ``max_seqlen_k``
     (optional) bounds cache_seqlens and sizes the context split; it defaults
-    to the block table's capacity.  Rows that see no key are 0.
+    to the block table's capacity; ``softmax_scale`` is positive and finite.
+    Rows that see no key are 0.
     """
     name = "d3d_verify_attn_paged_fp8" if causal else "d3d_draft_block_attn_fp8"
     return _attn(name, q, cache, cache_seqlens, block_table, softmax_scale, max_seqlen_k, out)

@@ -609,10 +609,11 @@ int d3d_kv_append_fp8(const void* k, const void* v, int64_t k_stride, int64_t v_
 /*
  * d3d_qk_rope_append over the 8-bit cache: q and k heads get RMSNorm over D
  * and rotate-half RoPE, q goes to q_out [T, Hq, 128] bf16, k and v into the
- * cache at slot_mapping[t].  Norm, rotation and scaling run in fp32 with one
- * rounding at the end (q to bf16, k to its code); angles positions[t] *
- * inv_freq[i] are reduced in 64 bits, so far positions lose nothing.  qkv, the
- * norm weights and q_out 8-byte aligned, inv_freq and parts 16-byte.
+ * cache at slot_mapping[t].  q runs in fp32 with one rounding to bf16 at the
+ * end, k in 64 bits with its result rounded to fp32 and to its code; angles
+ * positions[t] * inv_freq[i] are reduced in 64 bits, so far positions lose
+ * nothing.  qkv, the norm weights and q_out 8-byte aligned, inv_freq and parts
+ * 16-byte.
  * The _parts form takes qkv as the partials of d3d_gemm_rows64 (summed in
  * split order and rounded to bf16), as d3d_qk_rope_append_parts does.
  */
@@ -633,7 +634,8 @@ size_t d3d_attn_fp8_workspace_bytes(int B, int Q, int Hq, int Hkv, int D, int pa
 /*
  * Block attention over the 8-bit cache: d3d_verify_attn_paged,
  * d3d_draft_block_attn and d3d_packed_block_attn with the cache's codes and
- * scales.  q and out bf16, 16-byte aligned.  A row that sees no key is 0.  A key
+ * scales.  q and out bf16, 16-byte aligned; scale positive and finite
+ * (D3D_E_UNSUPPORTED otherwise).  A row that sees no key is 0.  A key
  * or value that holds a NaN reaches only the rows that see it; what lies
  * behind a context, in pages past it or in keys that a row does not see, has no
  * influence.  Page ids outside [0, num_pages) read as zero keys and values;

@@ -3,8 +3,7 @@
 * Appends of bf16 rows have one right answer, bit for bit: amax, the exponent
   and the rounding are exact in fp32.
 * After norm and rotation a value x is known to 2^-17 (|a| + |b|) of its rotated
-  pair (fp32 sums, rsqrt, and a hardware sine and cosine good to 2^-19 of the
-  turn's radius); a query adds half a bf16 step, 2^-8 |x|, a key half an e4m3 step,
+  pair (fp32 sums, rsqrt, sine and cosine); a query adds half a bf16 step, 2^-8 |x|, a key half an e4m3 step,
   2^-4 |x|, or 2^-10 of its scale below the normal range.
 * An attention output is off by half a bf16 step, 2^-8 |o|, and by the
   rounding of the probabilities to bf16 (each at most 2^-8 of itself) and fp32
@@ -295,6 +294,25 @@ def test_qk_rope_append_refusals():
             fp8_kv.qk_rope_append(**{**good, **bad})
 
 
+@pytest.mark.parametrize("n", (1, 3))
+def test_append_of_rows_at_odd_strides_and_addresses(n):
+    """Rows whose stride or address the kernel does not take, also of a single
+    token, whose stride no layout test looks at."""
+    g = _gen(61)
+    wide = torch.randn(8 * 1027, generator=g).to(BF)
+    slots = torch.tensor([5, 21, 40])[:n]
+    for at, step in ((0, 1027), (1, 1024), (2, 1026), (4, 1024), (3, 1025)):
+        rows = torch.as_strided(wide, (n, 8, D), (step, D, 1), at)
+        dev = torch.as_strided(wide.to(DEV), (n, 8, D), (step, D, 1), at)
+        got, want = (Fp8KV.empty(3, 16, 8, DEV) for _ in range(2))
+        fp8_kv.kv_append(dev, dev, got, slots.to(DEV))
+        fp8_kv.kv_append(rows.clone(memory_format=torch.contiguous_format).to(DEV), rows.to(DEV).clone(
+            memory_format=torch.contiguous_format), want, slots.to(DEV))
+        assert got.k.view(torch.uint8).any()
+        for a, b in ((got.k, want.k), (got.v, want.v), (got.k_scale, want.k_scale), (got.v_scale, want.v_scale)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # ------------------------------------------------------------------ attention
 def _close(out, ref, wgt):
     got = out.cpu().double()
@@ -469,7 +487,8 @@ def test_attention_arguments():
     for bad in (dict(q=q[0].to(DEV)), dict(q=q[..., :64].to(DEV)), dict(q=q[:, :, :7].to(DEV)),
                 dict(block_table=table[:1].to(DEV)), dict(cache_seqlens=lens[:1].to(DEV)), dict(max_seqlen_k=97),
                 dict(max_seqlen_k=0), dict(out=out.float()), dict(out=out[:1]),
-                dict(q=torch.zeros(2, 1, 130, D, dtype=BF, device=DEV))):
+                dict(q=torch.zeros(2, 1, 130, D, dtype=BF, device=DEV)), dict(softmax_scale=0.0),
+                dict(softmax_scale=-0.1), dict(softmax_scale=math.inf), dict(softmax_scale=math.nan)):
         with pytest.raises(ValueError):
             fp8_kv.flash_attn_with_kvcache(**{**good, **bad})
     vis = torch.tensor([[4, 0, 0]] * 4, dtype=torch.int32, device=DEV)

@@ -16,8 +16,8 @@
 //   new code = e4m3(x * 2^-e), |x| past 448 * 2^119 saturated, NaN and
 //     infinities as NaN (they do not count in amax)
 // A query is normalised and rotated in fp32 and rounded once, to bf16; a key in
-// 64 bits and rounded to fp32 and then to its code.  Angles are position *
-// inv_freq with the product and the whole turns taken off in 64 bits.
+// 64 bits and rounded once, to its code.  Angles are position * inv_freq with
+// the product and the whole turns taken off in 64 bits.
 //
 // A workgroup owns one (block, head): of the tokens of a call that fall into a
 // block the first in the list leads, its workgroup gathers the others
@@ -132,10 +132,36 @@ __device__ __forceinline__ void cos_sin(double p, float f, float& cs, float& sn)
     if (k & 2) sn = -sn;
 }
 
+// The same in 64 bits, with the sums' next terms below 2^-45 and 2^-49.
+__device__ __forceinline__ void cos_sin(double p, float f, double& cs, double& sn) {
+    double turns = p * (double)f;
+    turns = 4.0 * (turns - rint(turns));
+    const double q = rint(turns), x = (turns - q) * 1.57079632679489661923, z = x * x;
+    double s = 1.0 / 6227020800, c = -1.0 / 87178291200;
+    s = __builtin_fma(s, z, -1.0 / 39916800);
+    c = __builtin_fma(c, z, 1.0 / 479001600);
+    s = __builtin_fma(s, z, 1.0 / 362880);
+    c = __builtin_fma(c, z, -1.0 / 3628800);
+    s = __builtin_fma(s, z, -1.0 / 5040);
+    c = __builtin_fma(c, z, 1.0 / 40320);
+    s = __builtin_fma(s, z, 1.0 / 120);
+    c = __builtin_fma(c, z, -1.0 / 720);
+    s = __builtin_fma(s, z, -1.0 / 6);
+    c = __builtin_fma(c, z, 1.0 / 24);
+    s = __builtin_fma(x * z, s, x);
+    c = __builtin_fma(c, z, -0.5);
+    c = __builtin_fma(c, z, 1.0);
+    const int k = (int)q;
+    cs = (k & 1) ? s : c;
+    sn = (k & 1) ? c : s;
+    if ((k + 1) & 2) cs = -cs;
+    if (k & 2) sn = -sn;
+}
+
 constexpr double kTurn = 0.15915494309189533577;  // 1 / 2 pi
 
-template <int N>
-__device__ __forceinline__ void angles(const AppendParams& P, int64_t pos, int e, float* cs, float* sn) {
+template <int N, typename T>
+__device__ __forceinline__ void angles(const AppendParams& P, int64_t pos, int e, T* cs, T* sn) {
     const double p = (double)pos * kTurn;
 #pragma unroll
     for (int j = 0; j < N; ++j) cos_sin(p, P.inv_freq[e + j], cs[j], sn[j]);
@@ -166,11 +192,20 @@ __device__ __forceinline__ double xor_desc_d(double v) {
     return __builtin_bit_cast(double, hi << 32 | lo);
 }
 
+// x as a float rounded to odd: cut off, with the last bit set if anything was.  A
+// rounding of it to fewer bits, and a comparison, then comes out as x's own would.
+__device__ __forceinline__ float to_odd(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)u, kept = lo & 0xe0000000u;
+    const uint64_t v = (u >> 32 << 32) | ((lo & 0x1fffffffu) ? kept | 0x20000000u : kept);
+    return (float)__builtin_bit_cast(double, v);
+}
+
 // A key row's, over 16 lanes with 4 entries and their partners.  A key is
 // rounded to 4 bits, so a value next to a border falls to another code by any
 // error: the sum, the root (one Newton step on the hardware's) and the
 // rotation of x w, which a float holds exactly, run in 64 bits.
-__device__ __forceinline__ void norm_rotate_k(float* x, const float* w, const float* cs, const float* sn, float eps) {
+__device__ __forceinline__ void norm_rotate_k(float* x, const float* w, const double* cs, const double* sn, float eps) {
     double ss = 0.0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)x[j], (double)x[j], ss);
@@ -184,9 +219,8 @@ __device__ __forceinline__ void norm_rotate_k(float* x, const float* w, const fl
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const double a = (double)(x[j] * w[j]), b = (double)(x[4 + j] * w[4 + j]);
-        const double c = cs[j], s = sn[j];
-        x[j] = (float)((a * c - b * s) * r);
-        x[4 + j] = (float)((b * c + a * s) * r);
+        x[j] = to_odd((a * cs[j] - b * sn[j]) * r);
+        x[4 + j] = to_odd((b * cs[j] + a * sn[j]) * r);
     }
 }
 
@@ -349,7 +383,8 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
         // With one row per thread its angles stay, and the next heads' rows are on the
         // way while these are worked on; with more the registers do not reach.
         constexpr bool KEEP = IT == 1;
-        float cs[4], sn[4], w[8];
+        double cs[4], sn[4];
+        float w[8];
 #pragma unroll
         for (int it = 0; it < IT; ++it) m[it] = member[row16 + it * ROWS];
         if constexpr (ROPE) {

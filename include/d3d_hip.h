@@ -610,7 +610,7 @@ int d3d_kv_append_fp8(const void* k, const void* v, int64_t k_stride, int64_t v_
  * d3d_qk_rope_append over the 8-bit cache: q and k heads get RMSNorm over D
  * and rotate-half RoPE, q goes to q_out [T, Hq, 128] bf16, k and v into the
  * cache at slot_mapping[t].  q runs in fp32 with one rounding to bf16 at the
- * end, k in 64 bits with its result rounded to fp32 and to its code; angles
+ * end, k in 64 bits with one rounding to its code; angles
  * positions[t] * inv_freq[i] are reduced in 64 bits, so far positions lose
  * nothing.  qkv, the norm weights and q_out 8-byte aligned, inv_freq and parts
  * 16-byte.

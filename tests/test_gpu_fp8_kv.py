@@ -278,6 +278,28 @@ def test_qk_rope_append_of_split_products(T, splits):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
+@pytest.mark.parametrize("T,page,block,first", [(48, 16, 16, 0), (600, 16, 16, 4096), (600, 64, 64, 65536), (130, 256, 256, 256)])
+def test_rotated_keys_are_the_exact_ones(T, page, block, first):
+    """Normalised, rotated and scaled in 64 bits and rounded once, keys get the
+    codes of the formula: 2^-35 of a value, what 64-bit angles of these positions
+    leave, meets one of its 16 borders per octave at fewer than 1 in 10^8 values."""
+    g = _gen(T + page)
+    Hq, Hkv = 8, 8
+    qkv, qn, kn, inv_freq = _rope_inputs(g, T, Hq, Hkv)
+    pos = torch.arange(first, first + T)
+    P = -(-T // page)
+    slots = torch.randperm(P, generator=g)[torch.arange(T) // page] * page + torch.arange(T) % page
+    cache = Fp8KV.empty(P, page, Hkv, DEV, block=block)
+    before = of.from_bytes(cache.k, cache.v, cache.k_scale, cache.v_scale)
+    fp8_kv.qk_rope_append(*(t.to(DEV) for t in (qkv.view(T, -1), pos, qn, kn, inv_freq)), cache, slots.to(DEV), Hq, Hkv, 1e-6)
+    x = qkv.double()
+    rk, _ = of.norm_rotate(x[:, Hq:Hq + Hkv], kn, pos, inv_freq, 1e-6)
+    want = of.append(before, rk, x[:, Hq + Hkv:], slots)
+    got = of.from_bytes(cache.k, cache.v, cache.k_scale, cache.v_scale)
+    for n in ("k", "v", "k_exp", "v_exp"):
+        assert torch.equal(got[n], want[n]), n
+
+
 def test_qk_rope_append_refusals():
     g = _gen(1)
     qkv, qn, kn, inv_freq = (t.to(DEV) for t in _rope_inputs(g, 4, 4, 2))

@@ -30,6 +30,7 @@ HEAD_DIM = 128
 CODE = torch.float8_e4m3fn
 SCALE = torch.float8_e8m0fnu
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_NO_WORKSPACE = 256  # bytes asked for where one range per request leaves nothing to merge
 
 
 @dataclass(frozen=True, eq=False)
@@ -71,6 +72,8 @@ class Fp8KV:
         if any(t.device != self.k.device for t in (self.v, self.k_scale, self.v_scale)):
             raise ValueError("codes and scales must be on one device")
         object.__setattr__(self, "_index", self.k.get_device())
+        object.__setattr__(self, "_device", self.k.device)
+        object.__setattr__(self, "_dims", tuple(self.k.shape[:3]))
         object.__setattr__(self, "block", block)
 
     @classmethod
@@ -110,9 +113,12 @@ class Fp8KV:
 def _check_device(cache: Fp8KV, *tensors: Optional[torch.Tensor]) -> torch.device:
     """The cache's HIP device, which every given tensor must be on."""
     index = cache._index
-    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
+    if index < 0:
         _lib.require_device(cache.k, *tensors)  # raises, naming the devices
-    return cache.k.device
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _lib.require_device(cache.k, *tensors)
+    return cache._device
 
 
 def _rows(x: torch.Tensor, n: int, heads: int, name: str) -> torch.Tensor:
@@ -142,7 +148,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: Fp8KV, slot_mapping: torc
     """
     dev = _check_device(cache, k, v, slot_mapping)
     n = slot_mapping.numel()
-    P, H, ps, _ = cache.k.shape
+    P, H, ps = cache._dims
     k, v = _rows(k, n, H, "k"), _rows(v, n, H, "v")
     if slot_mapping.dtype is not torch.int64 or not slot_mapping.is_contiguous():
         slot_mapping = slot_mapping.to(torch.int64).contiguous()
@@ -167,7 +173,7 @@ def qk_rope_append(qkv: Product, positions: torch.Tensor, q_norm: torch.Tensor, 
     split = qkv if isinstance(qkv, SplitProduct) else None
     src = split.parts if split is not None else qkv
     dev = _check_device(cache, src, positions, q_norm, k_norm, inv_freq, slot_mapping, q_out)
-    P, H, ps, _ = cache.k.shape
+    P, H, ps = cache._dims
     if heads < 1 or kv_heads != H:
         raise ValueError("the cache's KV heads do not match the model's")
     width = (heads + 2 * kv_heads) * HEAD_DIM
@@ -176,25 +182,27 @@ def qk_rope_append(qkv: Product, positions: torch.Tensor, q_norm: torch.Tensor, 
     if src.shape[-1] != width:
         raise ValueError("qkv row width must be (heads + 2 kv_heads) * head_dim")
     T = src.shape[1] if split is not None else src.numel() // width
-    for t, name in ((positions, "positions"), (slot_mapping, "slot_mapping")):
-        if t.dtype is not torch.int64 or t.numel() != T or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous int64 with one entry per token")
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t.dtype is not torch.bfloat16 or t.numel() != HEAD_DIM or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous bf16 [{HEAD_DIM}]")
+    long, bf16 = torch.int64, torch.bfloat16
+    if positions.dtype is not long or positions.numel() != T or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int64 with one entry per token")
+    if slot_mapping.dtype is not long or slot_mapping.numel() != T or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
+    if q_norm.dtype is not bf16 or q_norm.numel() != HEAD_DIM or not q_norm.is_contiguous():
+        raise ValueError(f"q_norm must be contiguous bf16 [{HEAD_DIM}]")
+    if k_norm.dtype is not bf16 or k_norm.numel() != HEAD_DIM or not k_norm.is_contiguous():
+        raise ValueError(f"k_norm must be contiguous bf16 [{HEAD_DIM}]")
     if inv_freq.dtype is not torch.float32 or inv_freq.numel() != HEAD_DIM // 2 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be contiguous fp32 [head_dim / 2]")
     if q_out is None:
         q_out = torch.empty(T, heads, HEAD_DIM, dtype=torch.bfloat16, device=dev)
     elif q_out.dtype is not torch.bfloat16 or q_out.numel() != T * heads * HEAD_DIM or not q_out.is_contiguous():
         raise ValueError("q_out must be contiguous bf16 [T, heads, head_dim]")
-    tail = (positions.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
-            *cache._ptrs(), slot_mapping.data_ptr(), T, heads, kv_heads, HEAD_DIM, eps, ps, cache.block, P,
-            _lib.stream_ptr(dev))
-    if split is not None:
-        st = _lib.load().d3d_qk_rope_append_fp8_parts(src.data_ptr(), split.splits, *tail)
-    else:
-        st = _lib.load().d3d_qk_rope_append_fp8(src.data_ptr(), *tail)
+    lib = _lib.load()
+    call, head = ((lib.d3d_qk_rope_append_fp8, (src.data_ptr(),)) if split is None else
+                  (lib.d3d_qk_rope_append_fp8_parts, (src.data_ptr(), split.splits)))
+    st = call(*head, positions.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
+              *cache._ptrs(), slot_mapping.data_ptr(), T, heads, kv_heads, HEAD_DIM, eps, ps, cache.block, P,
+              _lib.stream_ptr(dev))
     if st:
         _lib.check(st, "d3d_qk_rope_append_fp8")
     return q_out
@@ -210,24 +218,26 @@ def _attn(fn_name: str, q, cache: Fp8KV, lens, block_table, softmax_scale, max_s
     if q.ndim != 4:
         raise ValueError("expected q [B, Q, Hq, D]")
     B, Q, Hq, D = q.shape
-    P, H, ps, _ = cache.k.shape
+    P, H, ps = cache._dims
     if D != HEAD_DIM or Hq % H:
         raise ValueError("q and cache head shapes are incompatible")
-    if block_table.ndim != 2 or block_table.shape[0] != B:
+    rows, max_pages = block_table.shape if block_table.ndim == 2 else (-1, 0)
+    if rows != B:
         raise ValueError("expected block_table [B, max_pages]")
     if lens.numel() != B:
         raise ValueError("expected one context length per request")
-    max_pages = block_table.shape[1]
     if max_seqlen_k is None:
         max_seqlen_k = max_pages * ps  # an upper bound that needs no host read
     else:
         max_seqlen_k = int(max_seqlen_k)
         if max_seqlen_k > max_pages * ps:
             raise ValueError("max_seqlen_k exceeds the block table's capacity")
-    if q.dtype is not torch.bfloat16 or not q.is_contiguous() or q.data_ptr() % 16:
+    q_ptr = q.data_ptr()
+    if q.dtype is not torch.bfloat16 or not q.is_contiguous() or q_ptr % 16:
         q = q.to(torch.bfloat16).contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
+        q_ptr = q.data_ptr()
     if block_table.dtype is not torch.int32 or not block_table.is_contiguous():
         block_table = block_table.to(torch.int32).contiguous()
     if lens.dtype is not torch.int32 or not lens.is_contiguous():
@@ -236,12 +246,14 @@ def _attn(fn_name: str, q, cache: Fp8KV, lens, block_table, softmax_scale, max_s
         out = torch.empty_like(q)
     elif out.dtype is not torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
         raise ValueError("out must be contiguous bf16 of q's shape")
-    ws = _lib.workspace(dev, "attn_fp8", _workspace_bytes(B, Q, Hq, H, ps, max_seqlen_k))
-    vis_args = () if vis is None else (vis.data_ptr(),)
+    ws_ptr, ws_bytes = None, _workspace_bytes(B, Q, Hq, H, ps, max_seqlen_k)
+    if ws_bytes > _NO_WORKSPACE:
+        ws = _lib.workspace(dev, "attn_fp8", ws_bytes)
+        ws_ptr = ws.data_ptr()
     st = getattr(_lib.load(), fn_name)(
-        q.data_ptr(), *cache._ptrs(), block_table.data_ptr(), lens.data_ptr(), *vis_args, out.data_ptr(), B, Q, Hq, H, D,
-        ps, cache.block, max_pages, P, _SCALE if softmax_scale is None else softmax_scale, max_seqlen_k,
-        ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
+        q_ptr, *cache._ptrs(), block_table.data_ptr(), lens.data_ptr(), *(() if vis is None else (vis.data_ptr(),)),
+        out.data_ptr(), B, Q, Hq, H, D, ps, cache.block, max_pages, P,
+        _SCALE if softmax_scale is None else softmax_scale, max_seqlen_k, ws_ptr, ws_bytes, _lib.stream_ptr(dev))
     if st:
         _lib.check(st, fn_name)
     return out

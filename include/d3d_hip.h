@@ -628,7 +628,8 @@ int d3d_qk_rope_append_fp8_parts(const float* parts, int splits, const int64_t* 
                                  void* stream);
 
 /* Bytes of workspace the attention calls over the 8-bit cache need; max_context
- * bounds every context_lens[b] and is passed to the call as well. */
+ * bounds every context_lens[b] and is passed to the call as well.  256 where the
+ * call needs none (a null workspace will do). */
 size_t d3d_attn_fp8_workspace_bytes(int B, int Q, int Hq, int Hkv, int D, int page_size, int max_context);
 
 /*

@@ -519,18 +519,31 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
                 }
             }
             first = false;
-            bf16x8 pop[RT];
+            // Probabilities as bf16 add 2^-9 of each; over many rows that is less than the
+            // results' own rounding.  A few rows (single tokens) may put all weight on two
+            // or three keys, where it showed (2.5 times the error of the result's rounding):
+            // there a second bf16 holds what the first leaves.  The products hide under the
+            // reads of a full card (48 requests of one token 43.6 us with either; one of
+            // 333 tokens 7.0 -> 7.5).
+            constexpr bool kTwo = RT == 1;
+            bf16x8 pop[RT], rest[kTwo ? RT : 1];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                uint32_t pw[4];
+                uint32_t pw[4], pr[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][i >> 1][2 * (i & 1)], P.scale_log2, -m[rt]));
                     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][i >> 1][2 * (i & 1) + 1], P.scale_log2, -m[rt]));
                     pw[i] = pack_bf16x2(p0, p1);
-                    // The sum takes the rounded probabilities, as the product does.
-                    l[rt] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw[i]), bf16x2{(__bf16)1.f, (__bf16)1.f}, l[rt], false);
+                    if constexpr (kTwo) {
+                        pr[i] = pack_bf16x2(p0 - __uint_as_float(pw[i] << 16), p1 - __uint_as_float(pw[i] & 0xffff0000u));
+                        l[rt] += p0 + p1;
+                    } else {
+                        // The sum takes the rounded probabilities, as the product does.
+                        l[rt] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw[i]), bf16x2{(__bf16)1.f, (__bf16)1.f}, l[rt], false);
+                    }
                 }
+                if constexpr (kTwo) rest[rt] = __builtin_bit_cast(bf16x8, u32x4{pr[0], pr[1], pr[2], pr[3]});
                 pop[rt] = __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -540,8 +553,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
                 const u32x2 c = lds_read_tr8(vbuf + (8 * g4 + (c16 >> 1)) * kVRow + 16 * n + 8 * (c16 & 1));
                 const bf16x8 vf = widen8(c[0], c[1], vs0, vs1);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+                for (int rt = 0; rt < RT; ++rt) {
                     o[rt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pop[rt], o[rt][n], 0, 0, 0);
+                    if constexpr (kTwo) o[rt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, rest[rt], o[rt][n], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();

@@ -31,6 +31,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace d3d {
 namespace fp8 {
@@ -48,12 +49,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
-// Up to this many tokens a workgroup takes one token and head, past it a window
-// of tokens and several heads (8 KV heads, rows of appended tokens in order:
-// 16 tokens 4.7 us against 7.7, 256 in blocks of 16 tokens 6.8 against 8.0,
-// but 12.5 against 9.7 in blocks of 64; 512 tokens 8.9 against 8.0 and 20.1
-// against 9.7, 1,024 13.9 against 8.2 and 36.1 against 10.6).
-constexpr int kFewTokens = 256;
+// Threads that the card holds at once.  While a workgroup per token and KV head
+// stays within them, that is the shortest chain; past it a workgroup takes a
+// window of tokens and several heads (8 KV heads, appended rows in order: blocks
+// of 16 tokens, 128 tokens 4.9 us against 5.9, 256 5.4 against 6.0, 400 7.3
+// against 6.1; blocks of 64, 64 tokens 6.8 against 8.5, 256 12.4 against 8.0).
+constexpr int64_t kCardThreads = 256 * 2048;
 constexpr float kMaxValue = 448.f * 0x1p119f;  // 448 * 2^kMaxExp
 
 struct AppendParams {
@@ -93,10 +94,15 @@ __device__ __forceinline__ void unpack4(u32x2 r, float* x) {
     x[3] = __uint_as_float(r[1] & 0xffff0000u);
 }
 
-// A row's entries of lane i of 16 as bf16: r[0] = 4i .. 4i + 3, r[1] = 64 + 4i ..
-template <bool PARTS>
+// A row's entries of lane i of 16 as bf16.  Rotating: r[0] = 4i .. 4i + 3, r[1] =
+// 64 + 4i .. , a pair's two in one lane; else 8i .. 8i + 7, one piece of memory.
+template <bool ROPE, bool PARTS>
 __device__ __forceinline__ void load_row(const uint16_t* src, const AppendParams& P, size_t e, int i, u32x2* r) {
-    if constexpr (PARTS) {
+    if constexpr (!ROPE) {
+        const u32x4_a8 v = *reinterpret_cast<const u32x4_a8*>(src + 8 * i);
+        r[0] = u32x2{v[0], v[1]};
+        r[1] = u32x2{v[2], v[3]};
+    } else if constexpr (PARTS) {
         f32x4 a = *reinterpret_cast<const f32x4*>(P.parts + e + 4 * i);
         f32x4 b = *reinterpret_cast<const f32x4*>(P.parts + e + 64 + 4 * i);
         for (int sp = 1; sp < P.splits; ++sp) {
@@ -272,11 +278,27 @@ __device__ __forceinline__ uint32_t quantise(u32x2 x, int e) {
     return __builtin_bit_cast(uint32_t, r);
 }
 
-// Four kept codes under a scale 2^d times finer (d = old - new <= 0).
+// Eight kept codes of a row under a scale 2^d times finer (f = 2^d, d <= 0).
 __device__ __forceinline__ uint32_t rescale(uint32_t c, float f) {
     const float y0 = __builtin_amdgcn_cvt_f32_fp8((int)c, 0), y1 = __builtin_amdgcn_cvt_f32_fp8((int)c, 1);
     const float y2 = __builtin_amdgcn_cvt_f32_fp8((int)c, 2), y3 = __builtin_amdgcn_cvt_f32_fp8((int)c, 3);
     return codes4(y0 * f, y1 * f, y2 * f, y3 * f);
+}
+__device__ __forceinline__ void rescale_row(uint8_t* row, int i, float f) {
+    u32x2* at = reinterpret_cast<u32x2*>(row) + i;
+    const u32x2 c = *at;
+    *at = u32x2{rescale(c[0], f), rescale(c[1], f)};
+}
+
+// Lane i's codes of a row: of the entries that load_row gave it.
+template <bool ROPE>
+__device__ __forceinline__ void put_codes(uint8_t* row, int i, uint32_t a, uint32_t b) {
+    if constexpr (ROPE) {
+        reinterpret_cast<uint32_t*>(row)[i] = a;
+        reinterpret_cast<uint32_t*>(row)[16 + i] = b;
+    } else {
+        reinterpret_cast<u32x2*>(row)[i] = u32x2{a, b};
+    }
 }
 
 // A query row's entries of lane i of 8: x[0..7] = 8i .., x[8..15] = 64 + 8i ...
@@ -303,9 +325,15 @@ __device__ __forceinline__ void load_row8(const uint16_t* src, const AppendParam
 }
 
 // HP heads at a time, each by NT / HP threads that take NT / HP / 16 slots of a
-// block at a time, IT times.
-template <int NT, int HP, int IT, bool ROPE, bool PARTS>
-__global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
+// block at a time, IT times.  MANY: two workgroups of 512 threads per CU, within
+// 128 registers (7,800 tokens of 32 + 8 heads 39 us, with 130 registers 48).
+//
+// What bounds it: many tokens, their bytes (that call's 176 MB at 4.5 TB/s; 14,688
+// tokens of 8 heads, 90 MB, 31 us at 2.9 TB/s: 459 windows are fewer than two per
+// CU, and more workgroups would each read the call's slots again).  Few, the chain
+// slots, block, rows, largest, codes (16 tokens of 32 + 8 heads 5.1 us).
+template <bool MANY, int NT, int HP, int IT, bool ROPE, bool PARTS>
+__global__ __launch_bounds__(NT, MANY ? 4 : 1) void append_kernel(AppendParams P) {
     const int tid = threadIdx.x, i16 = tid & 15;
     if constexpr (ROPE) {
         if ((int)blockIdx.x >= P.kv_groups) {
@@ -360,39 +388,65 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
         for (int j = tid; j < block; j += NT) member[j] = -1;
         __syncthreads();
         // One pass over the call's slots: its tokens of this block, wherever they stand.
-        // Sixteen loads at a time are on the way together (a loop of single loads:
-        // 42 us instead of 29 for 14,688 tokens of 8 heads).
+        // Up to sixteen loads at a time are on the way together (14,688 tokens: 42 -> 29
+        // us), and their slots are looked at one by one only where one of them is the
+        // block's (128 tokens of 8 heads 6.3 -> 5.4 us, 512 8.0 -> 6.1).
         bool before = false;
-        constexpr int kBatch = 16;
-        for (int j0 = tid; j0 < P.T; j0 += kBatch * NT) {
-            int64_t s[kBatch];
+        const uint64_t at = (uint64_t)blk << P.block_shift;
+        const uint32_t at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32), keep = ~(uint32_t)(block - 1);
+        const auto scan = [&](int j0, auto n, auto full) {
+            constexpr int N = decltype(n)::value;
+            uint32_t lo[N], hi[N], best = ~0u;
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) s[i] = j0 + i * NT < P.T ? P.slots[j0 + i * NT] : -1;
+            for (int i = 0; i < N; ++i) {  // behind the last token: the last one again, which changes nothing
+                const int j = j0 + i * NT + tid;
+                const uint64_t s = (uint64_t)P.slots[decltype(full)::value ? j : min(j, P.T - 1)];
+                lo[i] = (uint32_t)s;
+                hi[i] = (uint32_t)(s >> 32);
+            }
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (block_of(s[i]) == blk) {
-                    before |= j0 + i * NT < t;
-                    atomicMax(&member[(int)(s[i] & (block - 1))], j0 + i * NT);
+            for (int i = 0; i < N; ++i) best = min(best, ((lo[i] ^ at_lo) & keep) | (hi[i] ^ at_hi));
+            if (best == 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int j = min(j0 + i * NT + tid, P.T - 1);
+                    if ((((lo[i] ^ at_lo) & keep) | (hi[i] ^ at_hi)) == 0) {
+                        before |= j < t;
+                        atomicMax(&member[lo[i] & (block - 1)], j);
+                    }
                 }
-        }
+            }
+        };
+        int j0 = 0;
+        for (; P.T - j0 >= 16 * NT; j0 += 16 * NT) scan(j0, std::integral_constant<int, 16>{}, std::true_type{});
+        if (P.T - j0 > 4 * NT)
+            scan(j0, std::integral_constant<int, 16>{}, std::false_type{});
+        else if (P.T - j0 > NT)
+            scan(j0, std::integral_constant<int, 4>{}, std::false_type{});
+        else if (P.T > j0)
+            scan(j0, std::integral_constant<int, 1>{}, std::false_type{});
         if (__syncthreads_or(before)) continue;  // an earlier token leads this block
         const int64_t page = blk / per_page;
         const int nb = (int)(blk - page * per_page);
         const bool anew = member[0] >= 0;
         int m[IT];
+        bool some[IT];  // of the wave's rows one is written; of many tokens they mostly are, and asking costs registers
         // With one row per thread its angles stay, and the next heads' rows are on the
         // way while these are worked on; with more the registers do not reach.
-        constexpr bool KEEP = IT == 1;
+        constexpr bool KEEP = IT == 1, AHEAD = KEEP && MANY;
         double cs[4], sn[4];
         float w[8];
 #pragma unroll
-        for (int it = 0; it < IT; ++it) m[it] = member[row16 + it * ROWS];
+        for (int it = 0; it < IT; ++it) {
+            m[it] = member[row16 + it * ROWS];
+            some[it] = MANY || __any(m[it] >= 0);
+        }
         if constexpr (ROPE) {
             u32x2 r[2];
-            load_row<false>(P.kn, P, 0, i16, r);
+            load_row<true, false>(P.kn, P, 0, i16, r);
             unpack4(r[0], w);
             unpack4(r[1], w + 4);
-            if constexpr (KEEP) angles<4>(P, P.positions[max(m[0], 0)], 4 * i16, cs, sn);
+            if (KEEP && some[0]) angles<4>(P, P.positions[max(m[0], 0)], 4 * i16, cs, sn);
         }
         u32x2 raw[IT][4];
         int old_k = 0, old_v = 0;
@@ -403,18 +457,19 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
             old_v = P.v_scale[sc];
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
+                if (!some[it]) continue;
                 const size_t tm = (size_t)max(m[it], 0), e = (tm * (P.Hq + 2 * P.Hkv) + P.Hq + h) * D;
-                load_row<PARTS>(P.k + tm * P.k_stride + (size_t)h * D, P, e, i16, raw[it]);
-                load_row<PARTS>(P.v + tm * P.v_stride + (size_t)h * D, P, e + (size_t)P.Hkv * D, i16, raw[it] + 2);
+                load_row<ROPE, PARTS>(P.k + tm * P.k_stride + (size_t)h * D, P, e, i16, raw[it]);
+                load_row<ROPE, PARTS>(P.v + tm * P.v_stride + (size_t)h * D, P, e + (size_t)P.Hkv * D, i16, raw[it] + 2);
             }
         };
-        if constexpr (KEEP) fetch(head_at(h_first));
+        if constexpr (AHEAD) fetch(head_at(h_first));
         for (int hb = h_first; hb < h_last; hb += HP) {
             const bool here = hb + hp < h_last;
             const int h = head_at(hb);
             const size_t row0 = ((size_t)page * P.Hkv + h) * P.page_size + (size_t)nb * block;
             const size_t sc = ((size_t)page * P.Hkv + h) * per_page + nb;
-            if constexpr (!KEEP) fetch(h);
+            if constexpr (!AHEAD) fetch(h);
             float xk[ROPE ? IT : 1][8];
             u32x2 rk[IT][2], rv[IT][2];
 #pragma unroll
@@ -425,12 +480,13 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
                 rv[it][1] = raw[it][3];
             }
             const int was_k = min(old_k - 127, kMaxExp), was_v = min(old_v - 127, kMaxExp);
-            if constexpr (KEEP) {
+            if constexpr (AHEAD) {
                 if (hb + HP < h_last) fetch(head_at(hb + HP));
             }
             float ak = 0.f, av = 0.f;
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
+                if (!some[it]) continue;
                 float a, v = amax_bf16(rv[it]);
                 if constexpr (ROPE) {
                     unpack4(rk[it][0], xk[it]);
@@ -478,32 +534,21 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
                 const int r = row16 + it * ROWS;
-                uint32_t* dk = reinterpret_cast<uint32_t*>(P.k_cache + (row0 + r) * D) + i16;
-                uint32_t* dv = reinterpret_cast<uint32_t*>(P.v_cache + (row0 + r) * D) + i16;
+                uint8_t* dk = P.k_cache + (row0 + r) * D;
+                uint8_t* dv = P.v_cache + (row0 + r) * D;
                 if (!here) continue;
                 if (m[it] >= 0) {
-                    if constexpr (ROPE) {
-                        dk[0] = quantise(xk[it], ek);
-                        dk[16] = quantise(xk[it] + 4, ek);
-                    } else {
-                        dk[0] = quantise(rk[it][0], ek);
-                        dk[16] = quantise(rk[it][1], ek);
-                    }
-                    dv[0] = quantise(rv[it][0], ev);
-                    dv[16] = quantise(rv[it][1], ev);
+                    if constexpr (ROPE)
+                        put_codes<ROPE>(dk, i16, quantise(xk[it], ek), quantise(xk[it] + 4, ek));
+                    else
+                        put_codes<ROPE>(dk, i16, quantise(rk[it][0], ek), quantise(rk[it][1], ek));
+                    put_codes<ROPE>(dv, i16, quantise(rv[it][0], ev), quantise(rv[it][1], ev));
                 } else if (anew) {
-                    dk[0] = dk[16] = dv[0] = dv[16] = 0u;
+                    put_codes<ROPE>(dk, i16, 0u, 0u);
+                    put_codes<ROPE>(dv, i16, 0u, 0u);
                 } else {
-                    if (ek != was_k) {
-                        const uint32_t a = dk[0], b = dk[16];
-                        dk[0] = rescale(a, fk);
-                        dk[16] = rescale(b, fk);
-                    }
-                    if (ev != was_v) {
-                        const uint32_t a = dv[0], b = dv[16];
-                        dv[0] = rescale(a, fv);
-                        dv[16] = rescale(b, fv);
-                    }
+                    if (ek != was_k) rescale_row(dk, i16, fk);
+                    if (ev != was_v) rescale_row(dv, i16, fv);
                 }
             }
             // Every thread has read the old scales before this head's barrier.
@@ -516,17 +561,16 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendParams P) {
     }
 }
 
-template <int NT, int HP, int IT, bool ROPE, bool PARTS>
+template <bool MANY, int NT, int HP, int IT, bool ROPE, bool PARTS>
 static int launch(AppendParams& P, hipStream_t s) {
     // Few tokens: a workgroup per token and head, for the shortest chain.  Many:
     // windows of a block's tokens and all of a workgroup's heads in one pass over the
     // call's slots, split further while there are fewer workgroups than CUs.
-    const bool many = P.T > kFewTokens;
-    P.win = many ? std::min(1 << P.block_shift, 64) : 1;
+    P.win = MANY ? std::min(1 << P.block_shift, 64) : 1;
     const int64_t windows = ((int64_t)P.T + P.win - 1) / P.win;
     const int rounds = (P.Hkv + HP - 1) / HP;
-    P.kv_heads = many ? HP * (int)std::min<int64_t>(rounds, std::max<int64_t>(1, windows * rounds / 256)) : 1;
-    P.q_heads = many ? 8 : 1;
+    P.kv_heads = MANY ? HP * (int)std::min<int64_t>(rounds, std::max<int64_t>(1, windows * rounds / 256)) : 1;
+    P.q_heads = MANY ? 8 : 1;
     int64_t groups = windows * ((P.Hkv + P.kv_heads - 1) / P.kv_heads);
     if (groups > INT_MAX) return D3D_E_SHAPE;
     P.kv_groups = (int)groups;
@@ -535,7 +579,7 @@ static int launch(AppendParams& P, hipStream_t s) {
         groups += ((int64_t)P.T * chunks + NT / 8 - 1) / (NT / 8);
     }
     if (groups > (int64_t)UINT32_MAX / NT) return D3D_E_SHAPE;  // threads of a launch
-    hipLaunchKernelGGL((append_kernel<NT, HP, IT, ROPE, PARTS>), dim3((unsigned)groups), dim3(NT), 0, s, P);
+    hipLaunchKernelGGL((append_kernel<MANY, NT, HP, IT, ROPE, PARTS>), dim3((unsigned)groups), dim3(NT), 0, s, P);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? D3D_OK : (int)err;
 }
@@ -543,13 +587,18 @@ static int launch(AppendParams& P, hipStream_t s) {
 template <bool ROPE, bool PARTS>
 static int run(AppendParams& P, void* stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool many = P.T > kFewTokens;
+    const int threads = std::min(16 << P.block_shift, 1024);  // of a workgroup for one token and head
+    const bool many = (int64_t)P.T * P.Hkv * threads > kCardThreads;
     switch (P.block_shift) {
-        case 4: return many ? launch<512, 2, 1, ROPE, PARTS>(P, s) : launch<256, 1, 1, ROPE, PARTS>(P, s);
-        case 5: return launch<512, 1, 1, ROPE, PARTS>(P, s);
-        case 6: return launch<1024, 1, 1, ROPE, PARTS>(P, s);
-        case 7: return launch<1024, 1, 2, ROPE, PARTS>(P, s);
-        default: return launch<1024, 1, 4, ROPE, PARTS>(P, s);
+        case 4:
+            return many ? launch<true, 512, 2, 1, ROPE, PARTS>(P, s) : launch<false, 256, 1, 1, ROPE, PARTS>(P, s);
+        case 5: return many ? launch<true, 512, 1, 1, ROPE, PARTS>(P, s) : launch<false, 512, 1, 1, ROPE, PARTS>(P, s);
+        case 6:
+            return many ? launch<true, 1024, 1, 1, ROPE, PARTS>(P, s) : launch<false, 1024, 1, 1, ROPE, PARTS>(P, s);
+        case 7:
+            return many ? launch<true, 1024, 1, 2, ROPE, PARTS>(P, s) : launch<false, 1024, 1, 2, ROPE, PARTS>(P, s);
+        default:
+            return many ? launch<true, 1024, 1, 4, ROPE, PARTS>(P, s) : launch<false, 1024, 1, 4, ROPE, PARTS>(P, s);
     }
 }
 

@@ -108,6 +108,27 @@ def test_kv_append_many_tokens_across_windows():
         _same_cache(cache, of.append(of.from_bytes(*parts), k.double(), v.double(), s))
 
 
+@pytest.mark.parametrize("T,Hkv,page,block", [(300, 1, 16, 16), (1500, 1, 16, 16), (5000, 1, 64, 16), (9000, 1, 64, 32),
+                                              (700, 2, 64, 64), (2500, 1, 256, 256), (17000, 1, 128, 128)])
+def test_kv_append_of_scattered_calls(T, Hkv, page, block):
+    """Calls of every length class, their tokens in any order over blocks filled
+    before, some outside the cache and some slots twice."""
+    g = _gen(T)
+    P = T // page + 3
+    parts = _filled(g, P, Hkv, page, block)
+    slots = torch.randperm(P * page, generator=g)[:T]
+    slots[torch.randint(0, T, (T // 20,), generator=g)] = slots[0].clone()
+    slots[torch.randint(0, T, (T // 50,), generator=g)] = -1
+    slots[torch.randint(0, T, (T // 50,), generator=g)] = P * page
+    k, v = (torch.randn(T, Hkv, D, generator=g).to(BF) for _ in range(2))
+    cache = _to_dev(parts)
+    fp8_kv.kv_append(k.to(DEV), v.to(DEV), cache, slots.to(DEV))
+    want = of.append(of.from_bytes(*parts), k.double(), v.double(), slots)
+    got = of.from_bytes(cache.k, cache.v, cache.k_scale, cache.v_scale)
+    for n in ("k", "v", "k_exp", "v_exp"):
+        assert torch.equal(got[n], want[n]), n
+
+
 @pytest.mark.parametrize("block", [16, 64])
 def test_kv_append_token_by_token(block):
     """Growing, rewinding and starting a block anew, one call at a time."""
@@ -393,6 +414,22 @@ def test_attention_of_many_requests(lens):
 def test_attention_flat_and_peaked(sharp):
     """Equal scores, and scores whose largest outweighs everything."""
     _case(11, [1500, 77], 4, 8, 2, 16, 16, "causal", sharp=sharp)
+
+
+@pytest.mark.parametrize("Hq,Hkv,Q,n", [(8, 8, 1, 333), (16, 2, 1, 500), (32, 8, 2, 90), (16, 8, 8, 257)])
+def test_attention_of_few_rows_keeps_the_results_rounding(Hq, Hkv, Q, n):
+    """Up to 16 rows of a KV head over one range: probabilities are held to 2^-17
+    and fp32 scores (log2, below 2^8) to 2^-15, so that beside the result's half
+    step there is 2^-13 of the values at most, peaked rows included."""
+    g = _gen(n)
+    P = -(-n // 16) + 1
+    parts = _like_data(g, P, Hkv, 16, 16)
+    table = torch.randperm(P, generator=g)[None, :P].int()
+    for sharp in (1.0, 4.0, 12.0):
+        q = (torch.randn(1, Q, Hq, D, generator=g) * sharp).to(BF)
+        got = _attend(q, _to_dev(parts), [n], table, "causal").cpu().double()
+        ref, wgt = of.attention(q, of.from_bytes(*parts), table, [n], D ** -0.5)
+        assert bool(((got - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -13 * wgt).all())
 
 
 def test_attention_late_maximum():

@@ -55,6 +55,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // of 16 tokens, 128 tokens 4.9 us against 5.9, 256 5.4 against 6.0, 400 7.3
 // against 6.1; blocks of 64, 64 tokens 6.8 against 8.5, 256 12.4 against 8.0).
 constexpr int64_t kCardThreads = 256 * 2048;
+constexpr int kManyHeads = 8;   // query heads of a token that 8 lanes take, where tokens are many
 constexpr float kMaxValue = 448.f * 0x1p119f;  // 448 * 2^kMaxExp
 
 struct AppendParams {
@@ -83,7 +84,6 @@ struct AppendParams {
     int win;       // tokens per key / value workgroup, at most 64
     int kv_heads;  // KV heads per key / value workgroup
     int kv_groups; // workgroups of keys and values; queries follow
-    int q_heads;   // query heads per 8 lanes
 };
 
 // Entries 4i .. 4i + 3 of a bf16 row.
@@ -326,9 +326,9 @@ __device__ __forceinline__ void load_row8(const uint16_t* src, const AppendParam
 
 // HP heads at a time, each by NT / HP threads that take NT / HP / 16 slots of a
 // block at a time, IT times.  MANY: two workgroups of 512 threads per CU, within
-// 128 registers (7,800 tokens of 32 + 8 heads 39 us, with 130 registers 48).
+// 128 registers (7,800 tokens of 32 + 8 heads 38 us, with 130 registers 48).
 //
-// What bounds it: many tokens, their bytes (that call's 176 MB at 4.5 TB/s; 14,688
+// What bounds it: many tokens, their bytes (that call's 176 MB at 4.6 TB/s; 14,688
 // tokens of 8 heads, 90 MB, 31 us at 2.9 TB/s: 459 windows are fewer than two per
 // CU, and more workgroups would each read the call's slots again).  Few, the chain
 // slots, block, rows, largest, codes (16 tokens of 32 + 8 heads 5.1 us).
@@ -337,29 +337,38 @@ __global__ __launch_bounds__(NT, MANY ? 4 : 1) void append_kernel(AppendParams P
     const int tid = threadIdx.x, i16 = tid & 15;
     if constexpr (ROPE) {
         if ((int)blockIdx.x >= P.kv_groups) {
-            // Queries: 8 lanes take q_heads heads of one token.
+            // Queries: 8 lanes take QH heads of one token, QB rows on the way together (two
+            // 38.2 us for 7,800 tokens, one 39.2; four 38.5, eight run out of registers).
+            constexpr int QH = MANY ? kManyHeads : 1, QB = MANY ? 2 : 1;
             const int i8 = tid & 7;
-            const int chunks = (P.Hq + P.q_heads - 1) / P.q_heads;
+            const int chunks = (P.Hq + QH - 1) / QH;
             const int64_t g = (int64_t)((int)blockIdx.x - P.kv_groups) * (NT / 8) + (tid >> 3);
             const bool live = g < (int64_t)P.T * chunks;
-            const int t = live ? (int)(g / chunks) : 0, h0 = live ? (int)(g % chunks) * P.q_heads : 0;
+            const int t = live ? (int)(g / chunks) : 0, h0 = live ? (int)(g % chunks) * QH : 0;
             float cs[8], sn[8], w[16];
             angles<8>(P, P.positions[t], 8 * i8, cs, sn);
             load_row8<false>(P.qn, P, 0, i8, w);
-            const int n = min(P.q_heads, P.Hq - h0);
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) {
-                const size_t e = ((size_t)t * (P.Hq + 2 * P.Hkv) + h0 + j) * D;
-                float x[16];
-                load_row8<PARTS>(P.qkv + e, P, e, i8, x);
-                norm_rotate_q(x, w, cs, sn, P.eps);
-                if (live) {
-                    uint16_t* dst = P.q_out + ((size_t)t * P.Hq + h0 + j) * D + 8 * i8;
+            const int n = min(QH, P.Hq - h0);
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf)
-                        *reinterpret_cast<u32x4_a8*>(dst + 64 * hf) =
-                            u32x4_a8{pack2(x[8 * hf], x[8 * hf + 1]), pack2(x[8 * hf + 2], x[8 * hf + 3]),
-                                     pack2(x[8 * hf + 4], x[8 * hf + 5]), pack2(x[8 * hf + 6], x[8 * hf + 7])};
+            for (int jb = 0; jb < QH; jb += QB) {
+                float x[QB][16];
+#pragma unroll
+                for (int c = 0; c < QB; ++c) {  // behind the last head: the last one again, not written
+                    const size_t e = ((size_t)t * (P.Hq + 2 * P.Hkv) + h0 + min(jb + c, n - 1)) * D;
+                    load_row8<PARTS>(P.qkv + e, P, e, i8, x[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < QB; ++c) {
+                    norm_rotate_q(x[c], w, cs, sn, P.eps);
+                    if (live && jb + c < n) {
+                        uint16_t* dst = P.q_out + ((size_t)t * P.Hq + h0 + jb + c) * D + 8 * i8;
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const float* y = x[c] + 8 * hf;
+                            *reinterpret_cast<u32x4_a8*>(dst + 64 * hf) =
+                                u32x4_a8{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};
+                        }
+                    }
                 }
             }
             return;
@@ -570,12 +579,12 @@ static int launch(AppendParams& P, hipStream_t s) {
     const int64_t windows = ((int64_t)P.T + P.win - 1) / P.win;
     const int rounds = (P.Hkv + HP - 1) / HP;
     P.kv_heads = MANY ? HP * (int)std::min<int64_t>(rounds, std::max<int64_t>(1, windows * rounds / 256)) : 1;
-    P.q_heads = MANY ? 8 : 1;
     int64_t groups = windows * ((P.Hkv + P.kv_heads - 1) / P.kv_heads);
     if (groups > INT_MAX) return D3D_E_SHAPE;
     P.kv_groups = (int)groups;
     if (ROPE) {
-        const int64_t chunks = (P.Hq + P.q_heads - 1) / P.q_heads;
+        constexpr int QH = MANY ? kManyHeads : 1;
+        const int64_t chunks = (P.Hq + QH - 1) / QH;
         groups += ((int64_t)P.T * chunks + NT / 8 - 1) / (NT / 8);
     }
     if (groups > (int64_t)UINT32_MAX / NT) return D3D_E_SHAPE;  // threads of a launch

@@ -49,6 +49,7 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
+constexpr int NW = 4;           // waves of a workgroup
 constexpr int kStep = 32;       // tokens a wave takes at a time
 constexpr int kTile = 128;      // tokens four waves take at a time: the unit of ranges
 // Tiles per range from which four row tiles take two workgroups per CU: a short
@@ -220,7 +221,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
     return (hit >> 7) * 0xffu;
 }
 
-template <int MODE, int RT, int NW>
+template <int MODE, int RT>
 __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
     constexpr int NT = NW * 64, R = 16 * RT;
     constexpr int kGroups = kMaxTiles * kTile / 16;
@@ -475,12 +476,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnParams P) {
                     for (int sub = 0; sub < 2; ++sub)
                         sc[rt][sub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[sub][ks], qf, sc[rt][sub], 0, 0, 0);
                 }
-            // The next step's loads: not before the keys' registers are free (earlier
-            // the compiler spills them, and waits for them to do so: 131,072-token
-            // contexts 142 us instead of 104).  Behind the last step there is nothing to
-            // load, and a branch for it costs more than the last step's again (batch-8
-            // verify block 17.0 us instead of 16.3, prefill slices 487 instead of 475).
-            __builtin_amdgcn_sched_barrier(0);
+            // The next step's loads, behind the products that read the keys' registers.  Behind
+            // the last step there is nothing to load, and a branch for it costs more than the
+            // last step's again (batch-8 verify block 17.0 us instead of 16.3, prefill slices
+            // 487 instead of 475: the products move behind it, and registers run out).
             fetch_k(min(j + NW, steps - 1));
             fetch_v(min(j + NW, steps - 1));
             if (edge) {
@@ -839,9 +838,9 @@ static int attn_run(const void* q, const void* k_cache, const void* v_cache, con
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(pl.items * Hkv), (unsigned)pl.nqt);
     switch (pl.rt) {
-        case 1: hipLaunchKernelGGL((attn_kernel<MODE, 1, 4>), grid, dim3(256), 0, s, P); break;
-        case 2: hipLaunchKernelGGL((attn_kernel<MODE, 2, 4>), grid, dim3(256), 0, s, P); break;
-        default: hipLaunchKernelGGL((attn_kernel<MODE, 4, 4>), grid, dim3(256), 0, s, P); break;
+        case 1: hipLaunchKernelGGL((attn_kernel<MODE, 1>), grid, dim3(256), 0, s, P); break;
+        case 2: hipLaunchKernelGGL((attn_kernel<MODE, 2>), grid, dim3(256), 0, s, P); break;
+        default: hipLaunchKernelGGL((attn_kernel<MODE, 4>), grid, dim3(256), 0, s, P); break;
     }
     if (pl.merge) {
         const unsigned y = (unsigned)Hkv, z = (unsigned)(B * pl.nqt);

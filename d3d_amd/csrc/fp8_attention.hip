@@ -22,11 +22,11 @@
 // to the workspace and a second launch merges them.
 //
 // What bounds it, with measured times (32 query and 8 KV heads): long contexts
-// their bytes (two of 131,072 tokens, 16 queries: 103.7 us, 5.17 TB/s, the rate of
+// their bytes (two of 131,072 tokens, 16 queries: 102.3 us, 5.2 TB/s, the rate of
 // a large copy; 48 single tokens over 192 MB: 43.8 us); prompts the issue of about
-// 290 VALU (widening, exponentials, packing) beside 64 MFMA in a step of 64 rows (366
-// GFLOP in 410-470 us); small calls the chain of dependent loads and the second
-// launch (16 queries over 2,051 tokens: 9.2 + 4.0 us; one over 333: 7.4).
+// 250 VALU (widening, exponentials, packing) beside 64 MFMA in a step of 64 rows (366
+// GFLOP in 384 us); small calls the chain of dependent loads and the second
+// launch (16 queries over 2,051 tokens: 9.0 + 4.0 us; one over 333: 7.3).
 // Probabilities shared through LDS, the waves on their own output dimensions and a
 // barrier per 128 tokens, measured slower (573 us against 481 for the prompts).
 #include "fp8_cache.hpp"

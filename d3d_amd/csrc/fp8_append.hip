@@ -19,12 +19,12 @@
 // 64 bits and rounded once, to its code.  Angles are position * inv_freq with
 // the product and the whole turns taken off in 64 bits.
 //
-// A workgroup owns one (block, head): of the tokens of a call that fall into a
-// block the first in the list leads, its workgroup gathers the others
+// A (block, head) belongs to one workgroup: of the tokens of a call that fall
+// into a block the first in the list leads, its workgroup gathers the others
 // wherever they stand (the last of the same slot wins) and does everything
 // for the block, so nothing is raced for and results do not depend on order.
 // Sixteen lanes hold a row: lane i entries 4i .. 4i + 3 and 64 + 4i .. , the
-// pairs that the rotation mixes.
+// pairs that the rotation mixes, or 8i .. 8i + 7 where nothing is rotated.
 #include "fp8_cache.hpp"
 #include "../../include/d3d_hip.h"
 

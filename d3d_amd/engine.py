@@ -21,9 +21,10 @@ same constructor, methods and result dictionary:
 Keywords past the reference's (``device``, ``page_size``, ``mask_id``,
 ``use_graphs``, ``tuned_gemms``, ``kv_dtype``) choose the device, the KV page
 size, the draft's mask id, whether steps replay HIP graphs, whether both
-models' keys and values are kept in 8 bits (``kv_dtype="fp8"``: half the bytes,
-see fp8_kv; what a block is verified against then depends in the last bits
-on the blocks rejected before it), and whether the step's library GEMMs use the solution choices in gemm_tuned_gfx950.csv
+models' keys and values are kept in 8 bits (``kv_dtype="fp8"``: half the
+bytes, see fp8_kv; what a block is verified against then depends in the last
+bits on the blocks rejected before it), and whether the step's library GEMMs
+use the solution choices in gemm_tuned_gfx950.csv
 (``tuned_gemms=True``, off by default: gemm_tuning.enable turns on
 TunableOp, a process-wide torch switch, and ``close()`` turns it back; a
 no-op where the file's library versions or GPU do not match).

@@ -237,7 +237,7 @@ class Qwen3PagedModel(torch.nn.Module):
         attention, O GEMM, fused add + RMSNorm, gate-up GEMM, fused SiLU-mul,
         down GEMM (the decoder layer of serving/vendor/ssd/models/qwen3.py).
         Over an 8-bit cache (``kv.fp8``) the append quantises and the attention
-        reads the codes; norm and rotation then run in fp32 for both models.
+        reads the codes; norm and rotation are then the target's for both models.
         Blocks of at most 192 tokens run the projections on the
         weight-streaming HIP GEMM where layers.project / gate_up_silu pick it
         (when ``rows64_gemm``: the QKV, O and down GEMMs, whose K-split
